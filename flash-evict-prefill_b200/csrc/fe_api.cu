@@ -20,11 +20,13 @@
 #include <cstring>
 #include <mutex>
 
+#include "fe_decode.cuh"
 #include "fe_forward.cuh"
 #include "fe_gather.cuh"
 #include "fe_replay.cuh"
 #include "fe_select.cuh"
 #include "fe_snap.cuh"
+#include "fe_tree.cuh"
 
 namespace {
 
@@ -1017,3 +1019,5 @@ extern "C" int fe_evict_noalloc(const void* q, const int64_t* q_strides, const v
                   kv_heads, tokens, channels, dtype, causal, scale, recency_decay, observation_window, value_weighted,
                   budget, recent, pool_kernel, stream);
 }
+
+#include "fe_decode_host.cuh"

@@ -1,0 +1,145 @@
+// What the decode kernels share: the cache as the kernels see it and the even
+// split of all (row, key tile) work over the CTAs of one launch.
+//
+// A cache row (b, hkv) uses its first lengths[b*Hkv + hkv] slots.  The lengths
+// live on the device and change from step to step, so the host sizes a launch
+// by the capacity alone and the CTAs divide the real work among themselves:
+// the rows' key tiles, laid end to end, are cut into equal runs.  A run may
+// begin and end inside a row (a long row is shared by many CTAs, a batch of
+// short rows by few), which keeps every SM busy whatever the lengths are.
+#pragma once
+
+#include "fe_ptx.cuh"
+
+namespace fe {
+
+constexpr int DEC_TILE = 128;  // keys per tile
+
+__device__ __forceinline__ int cache_length(const int32_t* lengths, int bh, int capacity) {
+  return min(max(__ldg(lengths + bh), 0), capacity);
+}
+
+// One contiguous run of a row's tiles: tiles [j0, j1) of `tiles` for row tile mt.
+struct DecSegment {
+  int bh, mt, j0, j1, tiles, len;
+};
+
+// Walks the segments of one CTA's run.  A row bh has MT * tiles(bh) units (MT
+// row tiles of queries, each over all of the row's key tiles); tiles(bh) is
+// the cache's tiles and one tile of drafted tokens.
+struct DecWalk {
+  const int32_t* lengths;
+  int capacity, mts, bh, unit, left;
+  __device__ __forceinline__ bool next(DecSegment& s) {
+    if (left <= 0) return false;
+    s.bh = bh;
+    s.len = cache_length(lengths, bh, capacity);
+    s.tiles = (s.len + DEC_TILE - 1) / DEC_TILE + 1;
+    s.mt = unit / s.tiles;
+    s.j0 = unit - s.mt * s.tiles;
+    const int n = min(left, s.tiles - s.j0);
+    s.j1 = s.j0 + n;
+    left -= n;
+    unit += n;
+    if (unit == mts * s.tiles) {
+      unit = 0;
+      ++bh;
+    }
+    return true;
+  }
+};
+
+constexpr int DEC_SCRATCH_INTS = 36;
+
+// Where this CTA's run starts.  All THREADS threads call it; `scratch` is
+// shared memory.  With base != nullptr the first unit of every row and the
+// total are written there (nbh + 1 values).
+template <int THREADS>
+__device__ __forceinline__ DecWalk dec_walk_init(const int32_t* lengths, int nbh, int capacity, int mts, int cta,
+                                                 int nctas, int* scratch, int32_t* base) {
+  constexpr int WARPS = THREADS / 32;
+  static_assert(WARPS <= 32 && THREADS % 32 == 0, "one warp scans the warps' sums");
+  const int per_thread = (nbh + THREADS - 1) / THREADS;
+  const int first = min(nbh, static_cast<int>(threadIdx.x) * per_thread);
+  const int last = min(nbh, first + per_thread);
+  int mine = 0;
+  for (int i = first; i < last; ++i)
+    mine += mts * ((cache_length(lengths, i, capacity) + DEC_TILE - 1) / DEC_TILE + 1);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += n;
+  }
+  if (lane == 31) scratch[warp] = incl;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const int v = scratch[w];
+    before += w < warp ? v : 0;
+    total += v;
+  }
+  int start = before + incl - mine;
+  const int per = (total + nctas - 1) / nctas;
+  const int lo = min(total, cta * per);
+  for (int i = first; i < last; ++i) {
+    const int n = mts * ((cache_length(lengths, i, capacity) + DEC_TILE - 1) / DEC_TILE + 1);
+    if (base != nullptr) base[i] = start;
+    if (start <= lo && lo < start + n) {
+      scratch[33] = i;
+      scratch[34] = lo - start;
+    }
+    start += n;
+  }
+  if (base != nullptr && threadIdx.x == 0) base[nbh] = total;
+  __syncthreads();
+  DecWalk w;
+  w.lengths = lengths;
+  w.capacity = capacity;
+  w.mts = mts;
+  w.left = min(per, total - lo);
+  w.bh = w.left > 0 ? scratch[33] : 0;
+  w.unit = w.left > 0 ? scratch[34] : 0;
+  return w;
+}
+
+// Bytes of the 16-byte chunk `chunk` (8 elements) of row r in a 128-byte-swizzled
+// K-major tile whose 64-column groups are `group_bytes` apart.
+__device__ __forceinline__ uint32_t sw128_offset(int r, int chunk, int group_bytes) {
+  return static_cast<uint32_t>((chunk >> 3) * group_bytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+}
+
+// Eight consecutive channels of a row of 16-bit elements, zero past `channels`.
+// vec: the row is 16-byte aligned and channels is a multiple of 8.
+__device__ __forceinline__ uint4 load_row_chunk(const uint16_t* row, int chunk, int channels, bool vec) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  const int c = chunk * 8;
+  if (vec) {
+    if (c < channels) v = __ldg(reinterpret_cast<const uint4*>(row + c));
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = c + 2 * i < channels ? __ldg(row + c + 2 * i) : 0u;
+      const uint32_t hi = c + 2 * i + 1 < channels ? __ldg(row + c + 2 * i + 1) : 0u;
+      w[i] = lo | (hi << 16);
+    }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float elem_to_float(uint16_t x) {
+  if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(x) << 16);
+  else return __half2float(__ushort_as_half(x));
+}
+
+// Programmatic dependent launch: let the next kernel of the stream start
+// (its prologue only), and wait for the previous one's writes.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+}  // namespace fe

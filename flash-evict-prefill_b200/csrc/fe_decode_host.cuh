@@ -1,0 +1,215 @@
+// Host side of the decode entry points (included by fe_api.cu, whose checks,
+// tensor maps and error reporting it uses).
+#pragma once
+
+namespace {
+
+// Limits of the decode kernels: a tree's drafts are one key tile, and the query
+// heads of a KV head with one draft are at most two query tiles.
+constexpr int64_t kMaxDrafts = 128;
+constexpr int64_t kMaxGroup = 256;
+
+int sm_count(int dev) {
+  static std::atomic<int> cached[kMaxDevices];
+  if (dev < 0 || dev >= kMaxDevices) return 148;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
+    cached[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+int check_cache(const fe_cache* c) {
+  if (!c) return fail(FE_STATUS_INVALID, "null cache");
+  if (c->batch < 1 || c->kv_heads < 1 || c->capacity < 1 || c->channels < 1)
+    return fail(FE_STATUS_INVALID, "empty cache: batch=%lld kv_heads=%lld capacity=%lld channels=%lld",
+                (long long)c->batch, (long long)c->kv_heads, (long long)c->capacity, (long long)c->channels);
+  if (c->dtype != FE_DTYPE_F16 && c->dtype != FE_DTYPE_BF16) return fail(FE_STATUS_INVALID, "dtype must be f16 or bf16");
+  if (c->channels > 256) return fail(FE_STATUS_INVALID, "channels must be <= 256");
+  if (c->capacity > (int64_t(1) << 30) || c->batch * c->kv_heads > (int64_t(1) << 24))
+    return fail(FE_STATUS_UNSUPPORTED, "cache too large");
+  if (!c->k || !c->v || !c->lengths) return fail(FE_STATUS_INVALID, "null pointer");
+  return FE_STATUS_OK;
+}
+
+int check_drafts(const fe_cache* c, int64_t q_heads, int64_t drafts) {
+  if (q_heads < 1 || q_heads % c->kv_heads) return fail(FE_STATUS_INVALID, "q_heads must be divisible by kv_heads");
+  if (drafts < 1) return fail(FE_STATUS_INVALID, "at least one drafted token");
+  if (drafts > kMaxDrafts)
+    return fail(FE_STATUS_UNSUPPORTED, "at most %lld drafted tokens per call", (long long)kMaxDrafts);
+  if (q_heads / c->kv_heads > kMaxGroup)
+    return fail(FE_STATUS_UNSUPPORTED, "at most %lld query heads per KV head", (long long)kMaxGroup);
+  return FE_STATUS_OK;
+}
+
+// Rows of [batch, heads, tokens, channels] can be read 16 bytes at a time.
+bool rows_are_vectors(const void* p, const int64_t* s, int64_t batch, int64_t heads, int64_t tokens, int64_t channels) {
+  return channels % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && (batch == 1 || s[0] % 8 == 0) &&
+         (heads == 1 || s[1] % 8 == 0) && (tokens == 1 || s[2] % 8 == 0);
+}
+
+int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// Geometry of a tree-attention launch: a function of the shapes alone, so the
+// workspace query and the launch agree.
+struct TreeGeometry {
+  int rows, parts;  // query rows per work item, partials per run
+  bool dual;
+  int64_t M, MT, R, D4, ctas, slots, off_stats, off_acc, bytes;
+};
+
+int tree_geometry(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t drafts, int64_t capacity,
+                  int64_t channels, int sms, TreeGeometry* g) {
+  const int64_t nbh = batch * kv_heads;
+  g->M = q_heads / kv_heads * drafts;
+  g->dual = channels <= 128 && g->M > 128;
+  g->rows = g->dual ? 256 : 128;
+  g->parts = (channels <= 128 && !g->dual) ? 2 : 1;
+  g->MT = (g->M + g->rows - 1) / g->rows;
+  g->R = std::min<int64_t>(g->M, g->rows);
+  g->D4 = round_up(channels, 4);
+  const int64_t tiles = (capacity + fe::DEC_TILE - 1) / fe::DEC_TILE + 1;
+  if (nbh * g->MT * tiles > 0x3fffffff) return fail(FE_STATUS_UNSUPPORTED, "problem too large");
+  g->ctas = std::min<int64_t>(sms, nbh * g->MT * tiles);
+  g->slots = nbh * g->MT + g->ctas;
+  g->off_stats = round_up((nbh + 1) * 4, 256);
+  g->off_acc = g->off_stats + round_up(g->slots * g->parts * g->R * 8, 256);
+  g->bytes = g->off_acc + g->slots * g->parts * g->R * g->D4 * 4;
+  return FE_STATUS_OK;
+}
+
+template <typename Kern, typename... Args>
+int launch_dependent(Kern kern, dim3 grid, dim3 block, cudaStream_t stream, const char* what, Args... args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  return FE_STATUS_OK;
+}
+
+template <bool BF16, int DP, bool DUAL>
+int launch_tree(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn, const CUtensorMap& tvn,
+                const fe::TreeParams& p, cudaStream_t stream) {
+  using C = fe::TreeCfg<DP, DUAL>;
+  auto kern = fe::fe_tree_kernel<BF16, DP, DUAL>;
+  int rc = set_smem(kern, C::SMEM);
+  if (rc) return rc;
+  // setmaxnreg draws on the launch's own registers (see launch_fwd).
+  static std::atomic<int> checked_regs{0};
+  int regs = checked_regs.load(std::memory_order_relaxed);
+  if (regs == 0) {
+    cudaFuncAttributes fa;
+    cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
+    regs = fa.numRegs;
+    checked_regs.store(regs, std::memory_order_relaxed);
+  }
+  if (regs < fe::FWD_REGS_NEEDED)
+    return fail(FE_STATUS_UNSUPPORTED, "tree attention kernel compiled with %d registers/thread, needs %d", regs,
+                fe::FWD_REGS_NEEDED);
+  kern<<<dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, stream>>>(tk, tv, tkn, tvn, p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
+  const int64_t rows = (int64_t)p.B * p.Hkv * p.M;
+  constexpr int per_cta = fe::TREE_JOIN_THREADS / 32;
+  return launch_dependent(fe::fe_tree_join_kernel<BF16>, dim3((unsigned)((rows + per_cta - 1) / per_cta)),
+                          dim3(fe::TREE_JOIN_THREADS), stream, "tree join launch", p, C::PARTS, C::ROWS);
+}
+
+template <bool BF16>
+int launch_tree_dim(int dp, bool dual, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn,
+                    const CUtensorMap& tvn, const fe::TreeParams& p, cudaStream_t s) {
+  if (dp == 64) return dual ? launch_tree<BF16, 64, true>(tk, tv, tkn, tvn, p, s) : launch_tree<BF16, 64, false>(tk, tv, tkn, tvn, p, s);
+  if (dp == 128) return dual ? launch_tree<BF16, 128, true>(tk, tv, tkn, tvn, p, s) : launch_tree<BF16, 128, false>(tk, tv, tkn, tvn, p, s);
+  return launch_tree<BF16, 256, false>(tk, tv, tkn, tvn, p, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t fe_tree_workspace_bytes(const fe_cache* cache, int64_t q_heads, int64_t drafts) {
+  g_err[0] = 0;
+  if (check_cache(cache) || check_drafts(cache, q_heads, drafts)) return -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  TreeGeometry g;
+  if (tree_geometry(cache->batch, q_heads, cache->kv_heads, drafts, cache->capacity, cache->channels, sm_count(dev), &g))
+    return -1;
+  return g.bytes;
+}
+
+int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_strides, const void* k_new,
+                      const int64_t* k_new_strides, const void* v_new, const int64_t* v_new_strides,
+                      const uint8_t* tree, int64_t tree_batch_stride, void* out, float* lse, void* workspace,
+                      int64_t workspace_bytes, int64_t q_heads, int64_t drafts, float scale, void* stream) {
+  g_err[0] = 0;
+  int rc = check_cache(cache);
+  if (rc) return rc;
+  if ((rc = check_drafts(cache, q_heads, drafts))) return rc;
+  if (!q || !k_new || !v_new || !out || !lse || !workspace || !q_strides || !k_new_strides || !v_new_strides)
+    return fail(FE_STATUS_INVALID, "null pointer");
+  if (!std::isfinite(scale)) return fail(FE_STATUS_INVALID, "scale must be finite");
+  if (q_strides[3] != 1) return fail(FE_STATUS_UNSUPPORTED, "q: channel stride must be 1");
+  if (tree_batch_stride < 0) return fail(FE_STATUS_INVALID, "tree_batch_stride must be nonnegative");
+  if (reinterpret_cast<uintptr_t>(out) % 8 || reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(FE_STATUS_UNSUPPORTED, "out must be 8-byte and workspace 256-byte aligned");
+  int dev = 0;
+  if ((rc = enter(cache->k, stream, &dev))) return rc;
+  const int64_t B = cache->batch, H = cache->kv_heads, D = cache->channels;
+  TreeGeometry g;
+  if ((rc = tree_geometry(B, q_heads, H, drafts, cache->capacity, D, sm_count(dev), &g))) return rc;
+  if (workspace_bytes < g.bytes)
+    return fail(FE_STATUS_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)g.bytes);
+  CUtensorMap tk, tv, tkn, tvn;
+  if ((rc = make_map(&tk, cache->k, cache->k_strides, B, H, cache->capacity, D, cache->dtype, "cache k"))) return rc;
+  if ((rc = make_map(&tv, cache->v, cache->v_strides, B, H, cache->capacity, D, cache->dtype, "cache v"))) return rc;
+  if ((rc = make_map(&tkn, k_new, k_new_strides, B, H, drafts, D, cache->dtype, "k_new"))) return rc;
+  if ((rc = make_map(&tvn, v_new, v_new_strides, B, H, drafts, D, cache->dtype, "v_new"))) return rc;
+  fe::TreeParams p;
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_sb = q_strides[0], p.q_sh = q_strides[1], p.q_st = q_strides[2];
+  p.k_new = static_cast<const uint16_t*>(k_new);
+  p.kn_sb = k_new_strides[0], p.kn_sh = k_new_strides[1], p.kn_st = k_new_strides[2];
+  p.v_new = static_cast<const uint16_t*>(v_new);
+  p.vn_sb = v_new_strides[0], p.vn_sh = v_new_strides[1], p.vn_st = v_new_strides[2];
+  p.tree = tree;
+  p.tree_sb = tree_batch_stride;
+  p.lengths = cache->lengths;
+  p.out = static_cast<uint16_t*>(out);
+  p.lse = lse;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.base = reinterpret_cast<int32_t*>(ws);
+  p.stats = reinterpret_cast<float2*>(ws + g.off_stats);
+  p.acc = reinterpret_cast<float*>(ws + g.off_acc);
+  p.B = (int)B;
+  p.Hq = (int)q_heads;
+  p.Hkv = (int)H;
+  p.G = (int)(q_heads / H);
+  p.T = (int)drafts;
+  p.D = (int)D;
+  p.capacity = (int)cache->capacity;
+  p.M = (int)g.M;
+  p.MT = (int)g.MT;
+  p.R = (int)g.R;
+  p.D4 = (int)g.D4;
+  p.nctas = (int)g.ctas;
+  p.sc = (float)((double)scale * 1.4426950408889634);
+  p.q_vec = rows_are_vectors(q, q_strides, B, q_heads, drafts, D) ? 1 : 0;
+  p.timeout_ns = (uint64_t)g_watchdog_ns;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int dp = padded_dim(D);
+  return cache->dtype == FE_DTYPE_BF16 ? launch_tree_dim<true>(dp, g.dual, tk, tv, tkn, tvn, p, s)
+                                       : launch_tree_dim<false>(dp, g.dual, tk, tv, tkn, tvn, p, s);
+}
+
+}  // extern "C"

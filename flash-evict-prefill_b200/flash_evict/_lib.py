@@ -36,6 +36,16 @@ _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _F32 = ctypes.c_float
 
+
+class Cache(ctypes.Structure):
+    """fe_cache of include/flash_evict.h."""
+    _fields_ = [("k", _VP), ("v", _VP), ("k_strides", _I64 * 4), ("v_strides", _I64 * 4), ("mass", _VP),
+                ("norms", _VP), ("positions", _VP), ("lengths", _VP), ("batch", _I64), ("kv_heads", _I64),
+                ("capacity", _I64), ("channels", _I64), ("dtype", _INT)]
+
+
+_CACHEP = ctypes.POINTER(Cache)
+
 # name -> (restype, argtypes); mirrors include/flash_evict.h
 SIGNATURES = {
     "fe_attention_fwd": (_INT, [_VP, _I64P, _VP, _I64P, _VP, _I64P, _VP, _VP, _I64, _I64, _I64, _I64, _I64,
@@ -60,6 +70,9 @@ SIGNATURES = {
                               _I64, _VP]),
     "fe_evict_noalloc": (_INT, [_VP, _I64P, _VP, _I64P, _VP, _I64P, _VP, _VP, _VP, _VP, _I64, _I64, _I64,
                                 _I64, _I64, _INT, _INT, _F32, _F32, _I64, _INT, _I64, _I64, _I64, _VP]),
+    "fe_tree_workspace_bytes": (_I64, [_CACHEP, _I64, _I64]),
+    "fe_tree_attention": (_INT, [_CACHEP, _VP, _I64P, _VP, _I64P, _VP, _I64P, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64,
+                                 _F32, _VP]),
     "fe_device_status": (_INT, [_INT, _INT, ctypes.POINTER(_INT)]),
     "fe_set_watchdog_ns": (None, [_I64]),
     "fe_watchdog_selftest": (_INT, [_I64, _VP]),

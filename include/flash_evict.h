@@ -245,6 +245,50 @@ FE_API int fe_evict_noalloc(const void* q, const int64_t* q_strides, const void*
                             float recency_decay, int64_t observation_window, int value_weighted, int64_t budget,
                             int64_t recent, int64_t pool_kernel, void* stream);
 
+/* ---- Decode over a budgeted cache -----------------------------------------
+ * After the prefill has been evicted down to a budget, decoding attends to the
+ * kept tokens, adds each new token's attention weight to theirs, and evicts
+ * again when the cache grows past its budget.  No counterpart in the reference
+ * (its decoding is the kv_distill dependency's); the weights continue the
+ * importance of fe_replay_scores token by token.
+ *
+ * A cache row (b, h) holds lengths[b*kv_heads + h] tokens in its first slots,
+ * in any order (a token's K carries its rotary position).  k and v are
+ * [batch, kv_heads, capacity, channels] under the layout rules above; the
+ * bookkeeping arrays are contiguous [batch, kv_heads, capacity] and lengths
+ * contiguous [batch, kv_heads]; lengths are clamped to [0, capacity].  Slots
+ * past a row's length may hold anything.  mass, norms and positions may be
+ * NULL where an entry point does not use them. */
+typedef struct fe_cache {
+  void* k;
+  void* v;
+  int64_t k_strides[4];
+  int64_t v_strides[4];
+  float* mass;        /* accumulated attention weight                          */
+  float* norms;       /* ||v||_1 of the slot, or NULL: weights are not scaled  */
+  int32_t* positions; /* position of the token in its sequence                 */
+  int32_t* lengths;
+  int64_t batch, kv_heads, capacity, channels;
+  int dtype;
+} fe_cache;
+
+/* Attention of `drafts` (1..128) drafted tokens per sequence over the cache and
+ * over each other: draft t sees every cached token of its row and the drafts j
+ * with tree[b*tree_batch_stride + t*drafts + j] != 0 (tree == NULL: j <= t, a
+ * chain; tree_batch_stride 0: one mask for all sequences).  drafts == 1 with
+ * tree == NULL is an ordinary decode step.  The cache is not changed.
+ *   out: contiguous [batch, q_heads, drafts, channels], dtype of the cache;
+ *   lse: FP32 [batch, q_heads, drafts], the natural logarithm of the sum of
+ *   exp(scale * q.k) (-inf, with out 0, for a row that sees nothing).
+ * q needs channel stride 1; k_new and v_new follow the layout rules above.
+ * workspace: fe_tree_workspace_bytes() bytes on the cache's device, 256-byte
+ * aligned, contents irrelevant.  Two launches; bitwise reproducible. */
+FE_API int64_t fe_tree_workspace_bytes(const fe_cache* cache, int64_t q_heads, int64_t drafts);
+FE_API int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_strides, const void* k_new,
+                             const int64_t* k_new_strides, const void* v_new, const int64_t* v_new_strides,
+                             const uint8_t* tree, int64_t tree_batch_stride, void* out, float* lse, void* workspace,
+                             int64_t workspace_bytes, int64_t q_heads, int64_t drafts, float scale, void* stream);
+
 /* Read (and optionally clear) the device status word of `device`: the largest
  * FE_STATUS_* code any kernel raised since the last clear.  Synchronizes that
  * device; clearing also clears the device's host status word. */
