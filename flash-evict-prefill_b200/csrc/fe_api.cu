@@ -20,11 +20,13 @@
 #include <cstring>
 #include <mutex>
 
+#include "fe_commit.cuh"
 #include "fe_decode.cuh"
 #include "fe_forward.cuh"
 #include "fe_gather.cuh"
 #include "fe_replay.cuh"
 #include "fe_select.cuh"
+#include "fe_shrink.cuh"
 #include "fe_snap.cuh"
 #include "fe_tree.cuh"
 
@@ -147,6 +149,7 @@ const char* status_name(int code) {
   switch (code) {
     case FE_STATUS_TIMEOUT: return "device watchdog timeout";
     case FE_STATUS_BAD_INDEX: return "gather index out of range";
+    case FE_STATUS_CACHE_FULL: return "cache full, accepted tokens dropped";
     default: return "device error";
   }
 }

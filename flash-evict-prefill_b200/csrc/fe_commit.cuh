@@ -1,0 +1,473 @@
+// Commit of accepted drafts: their attention weight onto every cached token,
+// and their K/V rows onto the end of the cache (sm_100a).
+//
+// With the accepted drafts a_0..a_{n-1} of a sequence (in order) and the row
+// sums lse of their attention,
+//   w_i     = exp(-decay * (n-1-i))
+//   mass_k <- exp(-decay * n) * mass_k + norm_k * sum_{i,g} w_i exp(scale*q_{i,g}.k - lse_{i,g})
+// for cached tokens, the same sum over the accepted drafts that see it for each
+// appended token -- the importance of the prefill's replay, continued: the
+// weights are those it would give with the new tokens at the end.
+//
+// fe_commit_mass_kernel is key-stationary like the replay: S^T = K Q^T with the
+// 128 keys of a tile on the TMEM lanes and the accepted queries (n*G rows,
+// gathered and padded to 16) as columns, so each thread owns one key and sums
+// its row in registers: no shuffles, no atomics, one FP32 store per key.  What
+// bounds it is reading K once (2*D bytes a token).  The normaliser and weight
+// fold into one exponent bias per column: w exp(s - lse) = exp2(x*sc - bias).
+//
+// Work is split over the SMs as in fe_decode.cuh, the last tile of a row being
+// its drafts.  Four warpgroups take every fourth tile of a run, each with its
+// own 128-column S^T buffer; one warp streams K tiles by TMA, one issues the
+// products.  The queries of a run stay in shared memory; more than ROWS of
+// them take further launches.  fe_commit_append_kernel then writes the accepted
+// rows: a launch of its own because it changes the lengths that every CTA of
+// the first one reads.
+#pragma once
+
+#include "fe_decode.cuh"
+
+namespace fe {
+
+constexpr int COMMIT_MAX_ACCEPTED = 128;
+
+struct CommitParams {
+  const uint16_t* q;
+  int64_t q_sb, q_sh, q_st;
+  const float* lse;         // [B, Hq, T]
+  const int32_t* accepted;  // [B, A], negative: none
+  const uint8_t* tree;
+  int64_t tree_sb;
+  const int32_t* lengths;
+  const float* mass_in;
+  const float* norms_in;    // or null
+  const int32_t* pos_in;
+  float* mass_out;
+  float* norms_out;
+  int32_t* pos_out;
+  float* new_mass;     // workspace [B*Hkv, T]: summed weight of each draft
+  int32_t* old_lengths;  // workspace [B*Hkv]
+  int B, Hq, Hkv, G, T, A, D, capacity, nctas;
+  int row0;            // first query row (i*G + g) of this launch
+  int copy;            // mass_out, norms_out, pos_out are other buffers: fill them
+  float sc, decay_log2;
+  int q_vec;
+  uint64_t timeout_ns;
+};
+
+template <int DP>
+struct CommitCfg {
+  static constexpr int WGS = 4;
+  static constexpr int ROWS = DP <= 128 ? 256 : 128;  // query rows per launch
+  static constexpr int TILE = 128 * DP * 2;
+  static constexpr int NCH = DP / 64;
+  static constexpr int QTILES = ROWS / 128;
+  static constexpr int STAGES = DP <= 64 ? 8 : (DP <= 128 ? 4 : 2);
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = QTILES * TILE;
+  static constexpr int OFF_BIAS = OFF_K + STAGES * TILE;
+  static constexpr int OFF_MASK = OFF_BIAS + ROWS * 4;                       // uint32[128][4]
+  static constexpr int OFF_LIST = OFF_MASK + COMMIT_MAX_ACCEPTED * 16;      // int[128]
+  static constexpr int OFF_COL = OFF_LIST + COMMIT_MAX_ACCEPTED * 4;        // uint8[ROWS]
+  static constexpr int OFF_BAR = OFF_COL + ROWS;
+  // q_full, k_full[S], k_empty[S], s_full[WGS], s_free[WGS], drain
+  static constexpr int NBAR = 1 + 2 * STAGES + 2 * WGS + 1;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int SMEM = OFF_MISC + 16 + DEC_SCRATCH_INTS * 4 + 1024;
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
+  static constexpr int PRODUCER = WGS * 4;
+  static constexpr int ISSUER = WGS * 4 + 1;
+  static constexpr int THREADS = (WGS * 4 + 2) * 32;
+};
+
+// Number of accepted drafts of sequence b, by one converged warp; with list !=
+// nullptr their draft indices in order are written there.
+__device__ __forceinline__ int accepted_drafts(const int32_t* accepted, int A, int T, int b, int* list) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+  for (int a0 = 0; a0 < A; a0 += 32) {
+    const int j = a0 + lane < A ? __ldg(accepted + static_cast<int64_t>(b) * A + a0 + lane) : -1;
+    const bool valid = j >= 0 && j < T;
+    const uint32_t bal = __ballot_sync(0xffffffffu, valid);
+    if (valid && list != nullptr) list[n + __popc(bal & ((1u << lane) - 1u))] = j;
+    n += __popc(bal);
+  }
+  return n;
+}
+
+template <bool BF16, int DP>
+__global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
+    fe_commit_mass_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tkn,
+                          const __grid_constant__ CommitParams p) {
+  using C = CommitCfg<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* sbias = reinterpret_cast<float*>(smem + C::OFF_BIAS);
+  uint32_t* smask = reinterpret_cast<uint32_t*>(smem + C::OFF_MASK);
+  int* slist = reinterpret_cast<int*>(smem + C::OFF_LIST);
+  uint8_t* scol = smem + C::OFF_COL;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* k_full = q_full + 1;
+  uint64_t* k_empty = k_full + C::STAGES;
+  uint64_t* s_full = k_empty + C::STAGES;
+  uint64_t* s_free = s_full + C::WGS;
+  uint64_t* drain = s_free + C::WGS;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  int* scratch = reinterpret_cast<int*>(tmem_holder + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const uint32_t lane = threadIdx.x & 31;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    mbar_init(q_full, C::WGS * 4);
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int w = 0; w < C::WGS; ++w) {
+      mbar_init(&s_full[w], 1);
+      mbar_init(&s_free[w], 4);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == C::ISSUER) {
+    __syncwarp();
+    tmem_alloc(tmem_holder, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, 1, blockIdx.x, p.nctas, scratch, nullptr);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  const uint64_t TO = p.timeout_ns;
+  if (blockIdx.x == 0 && p.row0 == 0)
+    for (int i = threadIdx.x; i < p.B * p.Hkv; i += C::THREADS) p.old_lengths[i] = cache_length(p.lengths, i, p.capacity);
+  DecSegment sg;
+  auto rows_of = [&](int b, int n) { return min(max(n * p.G - p.row0, 0), C::ROWS); };
+
+  if (warp == C::PRODUCER) {
+    // ------------------------------------------------------------ producer --
+    if (lane == 0) {
+      tma_prefetch_desc(&tk);
+      tma_prefetch_desc(&tkn);
+    }
+    uint32_t it = 0;
+    bool ok = true;
+    while (ok && walk.next(sg)) {
+      const int b = sg.bh / p.Hkv, h = sg.bh - b * p.Hkv;
+      if (rows_of(b, accepted_drafts(p.accepted, p.A, p.T, b, nullptr)) == 0) continue;
+      for (int j = sg.j0; j < sg.j1; ++j) {
+        if (lane == 0) {
+          const int s = it % C::STAGES;
+          const uint32_t use = it / C::STAGES;
+          const bool drafts = j == sg.tiles - 1;
+          if (use > 0) ok = mbar_wait(&k_empty[s], (use - 1) & 1, TO, abort_flag);
+          if (ok) {
+            mbar_expect_tx(&k_full[s], C::TILE);
+            for (int c = 0; c < C::NCH; ++c)
+              tma_load_4d(smem + C::OFF_K + s * C::TILE + c * 16384, drafts ? &tkn : &tk, &k_full[s], c * 64,
+                          drafts ? 0 : j * DEC_TILE, h, b);
+          }
+        }
+        ok = warp_all(ok);
+        if (!ok) break;
+        ++it;
+      }
+    }
+    // Every load must have landed before the CTA exits.
+    if (lane == 0)
+      for (uint32_t i = it > C::STAGES ? it - C::STAGES : 0; i < it; ++i)
+        mbar_wait_inflight(&k_full[i % C::STAGES], (i / C::STAGES) & 1, TO);
+  } else if (warp == C::ISSUER) {
+    // ---------------------------------------------------------- MMA issuer --
+    const uint64_t dk = smem_desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024);
+    const uint64_t dq = smem_desc_sw128(smem_u32(smem + C::OFF_Q), 16, 1024);
+    const uint32_t dk_lo = static_cast<uint32_t>(dk), dk_hi = static_cast<uint32_t>(dk >> 32);
+    const uint32_t dq_lo = static_cast<uint32_t>(dq), dq_hi = static_cast<uint32_t>(dq >> 32);
+    uint32_t it0 = 0, nq = 0;
+    uint32_t used[C::WGS];
+    for (int w = 0; w < C::WGS; ++w) used[w] = 0;
+    bool ok = true;
+    while (ok && walk.next(sg)) {
+      const int b = sg.bh / p.Hkv;
+      const int rows = rows_of(b, accepted_drafts(p.accepted, p.A, p.T, b, nullptr));
+      if (rows == 0) continue;
+      const int ntile = sg.j1 - sg.j0;
+      if (lane == 0) {
+        ok = mbar_wait(q_full, nq & 1, TO, abort_flag);
+        tc_fence_after();
+        const int nch = (rows + 127) / 128;
+        // Rounds of one tile per warpgroup; the chunks of 128 queries inside.
+        for (int i0 = 0; i0 < ntile && ok; i0 += C::WGS)
+          for (int c = 0; c < nch && ok; ++c) {
+            const int cols = (min(rows - c * 128, 128) + 15) & ~15;
+            const uint32_t id = idesc_f16(128, cols, BF16, false);
+#pragma unroll
+            for (int w = 0; w < C::WGS; ++w) {
+              if (i0 + w >= ntile || !ok) continue;
+              const uint32_t tile = it0 + i0 + w;
+              const int s = tile % C::STAGES;
+              if (c == 0) ok = mbar_wait(&k_full[s], (tile / C::STAGES) & 1, TO, abort_flag);
+              if (ok && used[w] > 0) ok = mbar_wait(&s_free[w], (used[w] - 1) & 1, TO, abort_flag);
+              if (!ok) continue;
+              ++used[w];
+              tc_fence_after();
+              const uint32_t ka = dk_lo + static_cast<uint32_t>(s * (C::TILE >> 4));
+              const uint32_t qa = dq_lo + static_cast<uint32_t>(c * (C::TILE >> 4));
+#pragma unroll
+              for (int kk = 0; kk < DP / 16; ++kk) {
+                const uint32_t off = static_cast<uint32_t>(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
+                umma_ss_lohi(tmem + w * 128, ka + off, dk_hi, qa + off, dq_hi, id, kk > 0);
+              }
+              umma_commit(&s_full[w]);
+              if (c == nch - 1) umma_commit(&k_empty[s]);
+            }
+          }
+      }
+      ok = warp_all(ok);
+      it0 += ntile;
+      ++nq;
+    }
+    if (lane == 0) {
+      umma_commit(drain);
+      mbar_wait_inflight(drain, 0, TO);
+    }
+  } else {
+    // ------------------------------------------------ reduce (thread = key) --
+    const int wg = warp >> 2;
+    const int kr = ((warp & 3) << 5) + static_cast<int>(lane);
+    const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) << 5) << 16) + wg * 128;
+    const uint64_t sc2 = f2_pack(p.sc, p.sc);
+    const int tid = threadIdx.x;
+    constexpr int RT = C::WGS * 128;
+    uint32_t li = 0;
+    bool ok = true;
+    while (walk.next(sg)) {
+      const int b = sg.bh / p.Hkv, h = sg.bh - b * p.Hkv;
+      const int n = accepted_drafts(p.accepted, p.A, p.T, b, nullptr);
+      const int rows = rows_of(b, n);
+      const int ntile = sg.j1 - sg.j0;
+      const int i_first = p.row0 / p.G;
+      if (rows > 0) {
+        // Everyone is done with the previous run's queries (every product
+        // that read them has been waited for by the warpgroup it fed).
+        named_bar_sync(1, RT);
+        if (warp == 0) accepted_drafts(p.accepted, p.A, p.T, b, slist);
+        named_bar_sync(1, RT);
+        const int padded = (rows + 15) & ~15;
+        constexpr int CPR = DP / 8;
+        const uint16_t* qb = p.q + b * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
+        for (int i0 = tid; i0 < padded * CPR; i0 += RT * 4) {
+          uint4 v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * RT;
+            const int r = i / CPR;
+            v[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < rows) {
+              const int qi = (p.row0 + r) / p.G, g = p.row0 + r - qi * p.G;
+              v[u] = load_row_chunk(qb + g * p.q_sh + slist[qi] * p.q_st, i % CPR, p.D, p.q_vec);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + u * RT;
+            const int r = i / CPR;
+            if (r < padded)
+              *reinterpret_cast<uint4*>(smem + C::OFF_Q + (r >> 7) * C::TILE + sw128_offset(r & 127, i % CPR, 16384)) = v[u];
+          }
+        }
+        for (int r = tid; r < padded; r += RT) {
+          float bias = -INFINITY;  // padding, and rows that saw nothing, add 0
+          if (r < rows) {
+            const int qi = (p.row0 + r) / p.G, g = p.row0 + r - qi * p.G;
+            const float lse = __ldg(p.lse + (static_cast<int64_t>(b) * p.Hq + h * p.G + g) * p.T + slist[qi]);
+            if (lse != -INFINITY) bias = -fmaf(p.decay_log2, static_cast<float>(n - 1 - qi), lse * 1.4426950408889634f);
+            scol[r] = static_cast<uint8_t>(qi - i_first);
+          }
+          sbias[r] = bias;
+        }
+        if (sg.j1 == sg.tiles) {
+          // Which drafts each accepted query of this launch sees.
+          const int nq = (p.row0 + rows - 1) / p.G - i_first + 1;
+          for (int i = tid; i < nq * 4; i += RT) {
+            const int t = slist[i_first + (i >> 2)], w = i & 3;
+            const int cnt = min(max((p.tree == nullptr ? t + 1 : p.T) - 32 * w, 0), 32);
+            uint32_t bits = cnt == 32 ? 0xffffffffu : ((1u << cnt) - 1u);
+            if (p.tree != nullptr) {
+              const uint8_t* row = p.tree + b * p.tree_sb + static_cast<int64_t>(t) * p.T + 32 * w;
+              bits = 0u;
+#pragma unroll 8
+              for (int j = 0; j < cnt; ++j) bits |= (__ldg(row + j) != 0 ? 1u : 0u) << j;
+            }
+            smask[i] = bits;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+        named_bar_sync(1, RT);
+      }
+      const float fade = p.row0 == 0 ? exp2f(-p.decay_log2 * static_cast<float>(n)) : 1.0f;
+      const int nch = (rows + 127) / 128;
+      for (int i = wg; i < ntile; i += C::WGS) {
+        const int j = sg.j0 + i;
+        const bool drafts = j == sg.tiles - 1;
+        const int slot = j * DEC_TILE + kr;
+        const bool live = drafts ? kr < p.T : slot < sg.len;
+        const int64_t at = static_cast<int64_t>(sg.bh) * p.capacity + slot;
+        const int64_t at_new = static_cast<int64_t>(sg.bh) * p.T + kr;
+        float mass = 0.f, norm = 1.f;
+        if (live && !drafts) {
+          mass = p.row0 == 0 ? __ldg(p.mass_in + at) : p.mass_out[at];
+          if (p.norms_in != nullptr) norm = __ldg(p.norms_in + at);
+          if (p.copy && p.row0 == 0) {
+            p.pos_out[at] = __ldg(p.pos_in + at);
+            if (p.norms_out != nullptr) p.norms_out[at] = norm;
+          }
+        } else if (live && p.row0 > 0) {
+          mass = p.new_mass[at_new];
+        }
+        float total = 0.f;
+        for (int c = 0; c < nch && ok; ++c) {
+          ok = warp_all(mbar_wait(&s_full[wg], li & 1, TO, abort_flag));
+          if (!ok) break;
+          ++li;
+          tc_fence_after();
+          const int cols = (min(rows - c * 128, 128) + 15) & ~15;
+          uint64_t acc2[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) acc2[u] = 0ull;
+          for (int c0 = 0; c0 < cols; c0 += 16) {
+            float x[16];
+            tmem_ld16_nowait(tS + c0, reinterpret_cast<uint32_t*>(x));
+            tmem_wait_ld16(reinterpret_cast<uint32_t*>(x));
+            const float* bias = sbias + c * 128 + c0;
+#pragma unroll
+            for (int u = 0; u < 16; u += 2) {
+              const uint64_t a2 = f2_fma(f2_pack(x[u], x[u + 1]), sc2, f2_pack(bias[u], bias[u + 1]));
+              float a0, a1;
+              f2_unpack(a2, a0, a1);
+              if (drafts) {
+                // this thread's draft is seen by the column's query
+                const int r = c * 128 + c0 + u;
+                const uint32_t w0 = r < rows ? smask[scol[r] * 4 + (kr >> 5)] : 0u;
+                const uint32_t w1 = r + 1 < rows ? smask[scol[r + 1] * 4 + (kr >> 5)] : 0u;
+                if (!((w0 >> (kr & 31)) & 1u)) a0 = -INFINITY;
+                if (!((w1 >> (kr & 31)) & 1u)) a1 = -INFINITY;
+              }
+              acc2[(u >> 1) & 3] = f2_add(acc2[(u >> 1) & 3], f2_pack(ex2_approx(a0), ex2_approx(a1)));
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[wg]);
+          float s[8];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) f2_unpack(acc2[u], s[2 * u], s[2 * u + 1]);
+          total += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+        }
+        // Aborted (watchdog): the sum is incomplete; store NaN.
+        if (!ok) total = __int_as_float(0x7fffffff);
+        if (live) {
+          if (drafts) p.new_mass[at_new] = mass + total;
+          else p.mass_out[at] = fmaf(norm, total, mass * fade);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::ISSUER) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+struct AppendParams {
+  const uint16_t* k_new;
+  int64_t kn_sb, kn_sh, kn_st;
+  const uint16_t* v_new;
+  int64_t vn_sb, vn_sh, vn_st;
+  uint16_t* k;
+  int64_t k_sb, k_sh, k_st;
+  uint16_t* v;
+  int64_t v_sb, v_sh, v_st;
+  const int32_t* accepted;       // [B, A]
+  const int32_t* new_positions;  // [B, T]
+  const float* new_mass;
+  const int32_t* old_lengths;
+  float* mass;
+  float* norms;  // or null
+  int32_t* positions;
+  int32_t* lengths;
+  int Hkv, T, A, D, capacity;
+  int vec;  // rows can be moved 16 bytes at a time
+};
+
+constexpr int APPEND_THREADS = 128;
+
+// CTA (slice, kv head, sequence); a warp moves one accepted row at a time.
+template <bool BF16>
+__global__ void __launch_bounds__(APPEND_THREADS) fe_commit_append_kernel(const __grid_constant__ AppendParams p) {
+  __shared__ int list[COMMIT_MAX_ACCEPTED];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int bh = b * p.Hkv + h;
+  const int n = accepted_drafts(p.accepted, p.A, p.T, b, warp == 0 ? list : nullptr);
+  __syncthreads();
+  pdl_wait();
+  const int len = p.old_lengths[bh];
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.lengths[bh] = min(len + n, p.capacity);
+    if (len + n > p.capacity) raise_status(FE_STATUS_CACHE_FULL);
+    if (h == 0)
+      for (int a = 0; a < p.A; ++a)
+        if (p.accepted[static_cast<int64_t>(b) * p.A + a] >= p.T) raise_status(FE_STATUS_BAD_INDEX);
+  }
+  constexpr int WARPS = APPEND_THREADS / 32;
+  for (int i = blockIdx.x * WARPS + warp; i < n; i += gridDim.x * WARPS) {
+    const int slot = len + i;
+    if (slot >= p.capacity) break;
+    const int j = list[i];
+    const uint16_t* ks = p.k_new + b * p.kn_sb + h * p.kn_sh + j * p.kn_st;
+    const uint16_t* vs = p.v_new + b * p.vn_sb + h * p.vn_sh + j * p.vn_st;
+    uint16_t* kd = p.k + b * p.k_sb + h * p.k_sh + slot * p.k_st;
+    uint16_t* vd = p.v + b * p.v_sb + h * p.v_sh + slot * p.v_st;
+    float norm = 0.f;
+    if (p.vec) {
+      for (int c = lane * 8; c < p.D; c += 256) {
+        *reinterpret_cast<uint4*>(kd + c) = *reinterpret_cast<const uint4*>(ks + c);
+        const uint4 w = *reinterpret_cast<const uint4*>(vs + c);
+        *reinterpret_cast<uint4*>(vd + c) = w;
+        const uint16_t* e = reinterpret_cast<const uint16_t*>(&w);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) norm += fabsf(elem_to_float<BF16>(e[u]));
+      }
+    } else {
+      for (int c = lane; c < p.D; c += 32) {
+        kd[c] = ks[c];
+        const uint16_t e = vs[c];
+        vd[c] = e;
+        norm += fabsf(elem_to_float<BF16>(e));
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, o);
+    if (lane == 0) {
+      const int64_t at = static_cast<int64_t>(bh) * p.capacity + slot;
+      const float m = p.new_mass[static_cast<int64_t>(bh) * p.T + j];
+      p.mass[at] = p.norms != nullptr ? norm * m : m;
+      if (p.norms != nullptr) p.norms[at] = norm;
+      p.positions[at] = p.new_positions[static_cast<int64_t>(b) * p.T + j];
+    }
+  }
+}
+
+}  // namespace fe

@@ -213,3 +213,250 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
 }
 
 }  // extern "C"
+
+namespace {
+
+// The cache and the cache its updated bookkeeping goes to.
+int check_bookkeeping(const fe_cache* c, const fe_cache* out) {
+  int rc = check_cache(c);
+  if (rc) return rc;
+  if ((rc = check_cache(out))) return rc;
+  if (c->k != out->k || c->v != out->v || c->batch != out->batch || c->kv_heads != out->kv_heads ||
+      c->capacity != out->capacity || c->channels != out->channels || c->dtype != out->dtype)
+    return fail(FE_STATUS_INVALID, "out must be the same cache's k and v with other bookkeeping");
+  for (int i = 0; i < 4; ++i)
+    if (c->k_strides[i] != out->k_strides[i] || c->v_strides[i] != out->v_strides[i])
+      return fail(FE_STATUS_INVALID, "out must be the same cache's k and v with other bookkeeping");
+  if (!c->mass || !c->positions || !out->mass || !out->positions) return fail(FE_STATUS_INVALID, "the cache has no mass and positions");
+  if (!c->norms != !out->norms) return fail(FE_STATUS_INVALID, "norms must be given in both caches or in neither");
+  // Every array of its own or every array shared: a kernel writes one while it reads the other.
+  const bool shared = c->mass == out->mass;
+  if ((c->positions == out->positions) != shared || (c->lengths == out->lengths) != shared ||
+      (c->norms && (c->norms == out->norms) != shared))
+    return fail(FE_STATUS_INVALID, "out must share all of the cache's bookkeeping or none of it");
+  return FE_STATUS_OK;
+}
+
+int64_t commit_workspace(const fe_cache* c, int64_t drafts, int64_t* off_lengths) {
+  const int64_t nbh = c->batch * c->kv_heads;
+  *off_lengths = round_up(nbh * drafts * 4, 256);
+  return *off_lengths + nbh * 4;
+}
+
+template <bool BF16, int DP>
+int launch_commit(const CUtensorMap& tk, const CUtensorMap& tkn, fe::CommitParams p, cudaStream_t stream) {
+  using C = fe::CommitCfg<DP>;
+  auto kern = fe::fe_commit_mass_kernel<BF16, DP>;
+  int rc = set_smem(kern, C::SMEM);
+  if (rc) return rc;
+  // The accepted count is on the device; A is its most.
+  for (int64_t row0 = 0; row0 == 0 || row0 < (int64_t)p.A * p.G; row0 += C::ROWS) {
+    p.row0 = (int)row0;
+    kern<<<dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, stream>>>(tk, tkn, p);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "commit launch");
+  }
+  return FE_STATUS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t fe_commit_workspace_bytes(const fe_cache* cache, int64_t drafts) {
+  g_err[0] = 0;
+  if (check_cache(cache)) return -1;
+  if (drafts < 1 || drafts > kMaxDrafts) {
+    fail(FE_STATUS_INVALID, "drafts out of range");
+    return -1;
+  }
+  int64_t off;
+  return commit_workspace(cache, drafts, &off);
+}
+
+int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, const int64_t* q_strides,
+                     const void* k_new, const int64_t* k_new_strides, const void* v_new, const int64_t* v_new_strides,
+                     const uint8_t* tree, int64_t tree_batch_stride, const float* lse, const int32_t* accepted,
+                     int64_t max_accepted, const int32_t* new_positions, void* workspace, int64_t workspace_bytes,
+                     int64_t q_heads, int64_t drafts, float scale, float recency_decay, void* stream) {
+  g_err[0] = 0;
+  int rc = check_bookkeeping(cache, out);
+  if (rc) return rc;
+  if ((rc = check_drafts(cache, q_heads, drafts))) return rc;
+  if (max_accepted < 1 || max_accepted > fe::COMMIT_MAX_ACCEPTED)
+    return fail(FE_STATUS_INVALID, "max_accepted must be in [1, %d]", fe::COMMIT_MAX_ACCEPTED);
+  if (!q || !k_new || !v_new || !lse || !accepted || !new_positions || !workspace || !q_strides || !k_new_strides ||
+      !v_new_strides)
+    return fail(FE_STATUS_INVALID, "null pointer");
+  if (!std::isfinite(scale)) return fail(FE_STATUS_INVALID, "scale must be finite");
+  if (!std::isfinite(recency_decay) || recency_decay < 0)
+    return fail(FE_STATUS_INVALID, "recency_decay must be finite and nonnegative");
+  if (q_strides[3] != 1 || v_new_strides[3] != 1) return fail(FE_STATUS_UNSUPPORTED, "q and v_new: channel stride must be 1");
+  if (tree_batch_stride < 0) return fail(FE_STATUS_INVALID, "tree_batch_stride must be nonnegative");
+  const int64_t B = cache->batch, H = cache->kv_heads, D = cache->channels;
+  int64_t off_lengths;
+  if (workspace_bytes < commit_workspace(cache, drafts, &off_lengths))
+    return fail(FE_STATUS_INVALID, "workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 4) return fail(FE_STATUS_UNSUPPORTED, "workspace must be 4-byte aligned");
+  if (H > 65535 || B > 65535) return fail(FE_STATUS_UNSUPPORTED, "problem too large");
+  const int64_t units = B * H * ((cache->capacity + fe::DEC_TILE - 1) / fe::DEC_TILE + 1);
+  if (units > 0x3fffffff) return fail(FE_STATUS_UNSUPPORTED, "problem too large");
+  int dev = 0;
+  if ((rc = enter(cache->k, stream, &dev))) return rc;
+  CUtensorMap tk, tkn;
+  if ((rc = make_map(&tk, cache->k, cache->k_strides, B, H, cache->capacity, D, cache->dtype, "cache k"))) return rc;
+  if ((rc = make_map(&tkn, k_new, k_new_strides, B, H, drafts, D, cache->dtype, "k_new"))) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  fe::CommitParams p;
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_sb = q_strides[0], p.q_sh = q_strides[1], p.q_st = q_strides[2];
+  p.lse = lse;
+  p.accepted = accepted;
+  p.tree = tree;
+  p.tree_sb = tree_batch_stride;
+  p.lengths = cache->lengths;
+  p.mass_in = cache->mass;
+  p.norms_in = cache->norms;
+  p.pos_in = cache->positions;
+  p.mass_out = out->mass;
+  p.norms_out = out->norms;
+  p.pos_out = out->positions;
+  p.new_mass = reinterpret_cast<float*>(ws);
+  p.old_lengths = reinterpret_cast<int32_t*>(ws + off_lengths);
+  p.B = (int)B;
+  p.Hq = (int)q_heads;
+  p.Hkv = (int)H;
+  p.G = (int)(q_heads / H);
+  p.T = (int)drafts;
+  p.A = (int)max_accepted;
+  p.D = (int)D;
+  p.capacity = (int)cache->capacity;
+  p.nctas = (int)std::min<int64_t>(sm_count(dev), units);
+  p.row0 = 0;
+  p.copy = cache->mass != out->mass;
+  p.sc = (float)((double)scale * 1.4426950408889634);
+  p.decay_log2 = (float)((double)recency_decay * 1.4426950408889634);
+  p.q_vec = rows_are_vectors(q, q_strides, B, q_heads, drafts, D) ? 1 : 0;
+  p.timeout_ns = (uint64_t)g_watchdog_ns;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int dp = padded_dim(D);
+  const bool bf16 = cache->dtype == FE_DTYPE_BF16;
+  rc = bf16 ? (dp == 64 ? launch_commit<true, 64>(tk, tkn, p, s)
+                        : dp == 128 ? launch_commit<true, 128>(tk, tkn, p, s) : launch_commit<true, 256>(tk, tkn, p, s))
+            : (dp == 64 ? launch_commit<false, 64>(tk, tkn, p, s)
+                        : dp == 128 ? launch_commit<false, 128>(tk, tkn, p, s) : launch_commit<false, 256>(tk, tkn, p, s));
+  if (rc) return rc;
+  fe::AppendParams a;
+  a.k_new = static_cast<const uint16_t*>(k_new);
+  a.kn_sb = k_new_strides[0], a.kn_sh = k_new_strides[1], a.kn_st = k_new_strides[2];
+  a.v_new = static_cast<const uint16_t*>(v_new);
+  a.vn_sb = v_new_strides[0], a.vn_sh = v_new_strides[1], a.vn_st = v_new_strides[2];
+  a.k = static_cast<uint16_t*>(cache->k);
+  a.k_sb = cache->k_strides[0], a.k_sh = cache->k_strides[1], a.k_st = cache->k_strides[2];
+  a.v = static_cast<uint16_t*>(cache->v);
+  a.v_sb = cache->v_strides[0], a.v_sh = cache->v_strides[1], a.v_st = cache->v_strides[2];
+  a.accepted = accepted;
+  a.new_positions = new_positions;
+  a.new_mass = p.new_mass;
+  a.old_lengths = p.old_lengths;
+  a.mass = out->mass;
+  a.norms = out->norms;
+  a.positions = out->positions;
+  a.lengths = out->lengths;
+  a.Hkv = p.Hkv;
+  a.T = p.T;
+  a.A = p.A;
+  a.D = p.D;
+  a.capacity = p.capacity;
+  a.vec = rows_are_vectors(k_new, k_new_strides, B, H, drafts, D) && rows_are_vectors(v_new, v_new_strides, B, H, drafts, D) &&
+          rows_are_vectors(cache->k, cache->k_strides, B, H, cache->capacity, D) &&
+          rows_are_vectors(cache->v, cache->v_strides, B, H, cache->capacity, D);
+  const dim3 grid((unsigned)((max_accepted + 3) / 4), (unsigned)H, (unsigned)B);
+  return bf16 ? launch_dependent(fe::fe_commit_append_kernel<true>, grid, dim3(fe::APPEND_THREADS), s, "append launch", a)
+              : launch_dependent(fe::fe_commit_append_kernel<false>, grid, dim3(fe::APPEND_THREADS), s, "append launch", a);
+}
+
+int64_t fe_evict_workspace_bytes(const fe_cache* cache, int64_t budget) {
+  g_err[0] = 0;
+  if (check_cache(cache)) return -1;
+  if (budget < 1) {
+    fail(FE_STATUS_INVALID, "budget must be positive");
+    return -1;
+  }
+  // Holes and movers of every row: no more than either side of the budget.
+  const int64_t list = std::max<int64_t>(1, std::min(budget, cache->capacity - budget));
+  return cache->batch * cache->kv_heads * list * 8;
+}
+
+int fe_evict_tokens(const fe_cache* cache, const fe_cache* out, int64_t budget, int64_t recent, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  int rc = check_bookkeeping(cache, out);
+  if (rc) return rc;
+  if (budget < 1) return fail(FE_STATUS_INVALID, "budget must be positive");
+  if (recent < 0 || recent > budget) return fail(FE_STATUS_INVALID, "recent must be an integer in [0, budget]");
+  if (!workspace) return fail(FE_STATUS_INVALID, "null pointer");
+  const int64_t rows = cache->batch * cache->kv_heads, cap = cache->capacity;
+  const int64_t list = std::max<int64_t>(1, std::min(budget, cap - budget));
+  if (workspace_bytes < rows * list * 8) return fail(FE_STATUS_INVALID, "workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 4) return fail(FE_STATUS_UNSUPPORTED, "workspace must be 4-byte aligned");
+  for (const int64_t* s : {cache->k_strides, cache->v_strides}) {
+    if (s[3] != 1) return fail(FE_STATUS_UNSUPPORTED, "cache: channel stride must be 1");
+    for (int i = 0; i < 3; ++i)
+      if (s[i] < 0 || s[i] % 8) return fail(FE_STATUS_UNSUPPORTED, "cache: strides must be multiples of 8");
+  }
+  if (reinterpret_cast<uintptr_t>(cache->k) % 16 || reinterpret_cast<uintptr_t>(cache->v) % 16)
+    return fail(FE_STATUS_UNSUPPORTED, "cache: base pointers must be 16-byte aligned");
+  int dev = 0;
+  if ((rc = enter(cache->k, stream, &dev))) return rc;
+  if (budget >= cap && cache->mass == out->mass) return FE_STATUS_OK;  // nothing can be over the budget
+  fe::ShrinkParams p;
+  p.k = static_cast<uint8_t*>(cache->k);
+  p.k_sb = cache->k_strides[0] * 2, p.k_sh = cache->k_strides[1] * 2, p.k_st = cache->k_strides[2] * 2;
+  p.v = static_cast<uint8_t*>(cache->v);
+  p.v_sb = cache->v_strides[0] * 2, p.v_sh = cache->v_strides[1] * 2, p.v_st = cache->v_strides[2] * 2;
+  p.mass_in = cache->mass;
+  p.norms_in = cache->norms;
+  p.pos_in = cache->positions;
+  p.len_in = cache->lengths;
+  p.mass_out = out->mass;
+  p.norms_out = out->norms;
+  p.pos_out = out->positions;
+  p.len_out = out->lengths;
+  p.holes = static_cast<int32_t*>(workspace);
+  p.movers = p.holes + rows * list;
+  p.list = list;
+  p.Hkv = (int)cache->kv_heads;
+  p.capacity = (int)cap;
+  p.budget = (int)std::min(budget, cap);
+  p.recent = (int)std::min<int64_t>(recent, 0x7fffffff);
+  p.row_bytes = (int)cache->channels * 2;
+  p.copy = cache->mass != out->mass;
+  // CTAs per row: enough to fill the SMs with few rows, at least 1024 keys each.
+  int cl = 1;
+  while (cl < 8 && rows * cl < sm_count(dev) && cap / (2 * cl) >= 1024) cl *= 2;
+  const int64_t wlen = ((cap + cl * fe::SHRINK_WARPS - 1) / (cl * fe::SHRINK_WARPS) + 31) / 32 * 32;
+  const bool smem_keys = wlen * fe::SHRINK_WARPS <= fe::SHRINK_SMEM_KEYS;
+  auto kern = smem_keys ? fe::fe_shrink_kernel<true> : fe::fe_shrink_kernel<false>;
+  const int smem = smem_keys ? (int)(wlen * fe::SHRINK_WARPS * 4) : 0;
+  if ((rc = set_smem(kern, smem < 49152 ? 49152 : smem))) return rc;
+  if (rows * cl > 0x7fffffff) return fail(FE_STATUS_UNSUPPORTED, "too many rows");
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)(rows * cl));
+  cfg.blockDim = dim3(fe::SHRINK_THREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cl;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) return cuda_fail(e, "cache eviction launch");
+  return FE_STATUS_OK;
+}
+
+}  // extern "C"

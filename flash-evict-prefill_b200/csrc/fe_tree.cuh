@@ -70,6 +70,7 @@ struct TreeCfg {
   static constexpr int NBAR = 1 + 4 * STAGES + 7;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_MISC + 16 + 32 + DEC_SCRATCH_INTS * 4 + 1024;
+  static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int THREADS = 384;
 };
 

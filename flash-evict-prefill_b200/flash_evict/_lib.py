@@ -18,6 +18,7 @@ STATUS_UNSUPPORTED = 2
 STATUS_CUDA = 3
 STATUS_TIMEOUT = 4
 STATUS_BAD_INDEX = 5
+STATUS_CACHE_FULL = 6
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
 QUERY_BLOCK = 256
@@ -28,6 +29,7 @@ _STATUS_NAMES = {
     STATUS_CUDA: "CUDA error",
     STATUS_TIMEOUT: "device watchdog timeout",
     STATUS_BAD_INDEX: "gather index out of range",
+    STATUS_CACHE_FULL: "cache full, accepted tokens dropped",
 }
 
 _I64P = ctypes.POINTER(ctypes.c_int64)
@@ -73,6 +75,11 @@ SIGNATURES = {
     "fe_tree_workspace_bytes": (_I64, [_CACHEP, _I64, _I64]),
     "fe_tree_attention": (_INT, [_CACHEP, _VP, _I64P, _VP, _I64P, _VP, _I64P, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64,
                                  _F32, _VP]),
+    "fe_commit_workspace_bytes": (_I64, [_CACHEP, _I64]),
+    "fe_commit_tokens": (_INT, [_CACHEP, _CACHEP, _VP, _I64P, _VP, _I64P, _VP, _I64P, _VP, _I64, _VP, _VP, _I64, _VP, _VP,
+                                _I64, _I64, _I64, _F32, _F32, _VP]),
+    "fe_evict_workspace_bytes": (_I64, [_CACHEP, _I64]),
+    "fe_evict_tokens": (_INT, [_CACHEP, _CACHEP, _I64, _I64, _VP, _I64, _VP]),
     "fe_device_status": (_INT, [_INT, _INT, ctypes.POINTER(_INT)]),
     "fe_set_watchdog_ns": (None, [_I64]),
     "fe_watchdog_selftest": (_INT, [_I64, _VP]),

@@ -7,6 +7,12 @@ on the device, so a step can be captured in a CUDA graph):
 
   tree_attention(q, k_new, v_new, cache, tree=...)  -> fe_tree_attention
       drafted tokens (one: an ordinary step) attend to the cache and to each other
+  commit_tokens(cache, q, k_new, v_new, lse, accepted, positions)
+                                                    -> fe_commit_tokens
+      the accepted drafts' attention weight is added to every cached token's, and
+      their K/V rows to the cache
+  evict_tokens(cache, budget, recent=...)           -> fe_evict_tokens
+      rows over their budget lose the tokens of least weight, in place
 """
 import ctypes
 import math
@@ -16,7 +22,7 @@ import torch
 from . import _lib
 from .prefill import _tma_view
 
-__all__ = ["KVCache", "tree_attention", "MAX_DRAFTS"]
+__all__ = ["KVCache", "tree_attention", "commit_tokens", "evict_tokens", "MAX_DRAFTS"]
 
 MAX_DRAFTS = 128
 
@@ -176,3 +182,88 @@ def tree_attention(q, k_new, v_new, cache, *, tree=None, scale=None):
           v_new.data_ptr(), _strides(v_new), None if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(),
           lse.data_ptr(), workspace.data_ptr(), size, hq, t, scale)
     return out, lse
+
+
+def _check_out(cache, out):
+    if cache.mass is None:
+        raise ValueError("the cache has no mass and positions")
+    if out is None or out is cache:
+        return cache
+    shares = [a is not None and a.data_ptr() == b.data_ptr() for a, b in ((cache.mass, out.mass), (cache.positions, out.positions),
+                                                                          (cache.lengths, out.lengths)) if b is not None]
+    if out.mass is None or (out.norms is None) != (cache.norms is None) or any(shares):
+        raise ValueError("out needs bookkeeping tensors of its own, the same ones that the cache has")
+    if cache.k.data_ptr() != out.k.data_ptr() or cache.v.data_ptr() != out.v.data_ptr() or cache.k.shape != out.k.shape \
+            or cache.k.dtype != out.k.dtype or cache.k.stride() != out.k.stride() or cache.v.stride() != out.v.stride():
+        raise ValueError("out must hold the cache's own k and v")
+    return out
+
+
+def commit_tokens(cache, q, k_new, v_new, lse, accepted, positions, *, tree=None, scale=None, recency_decay=0., out=None):
+    """Add accepted drafts to the cache; returns the cache with the updated bookkeeping.
+
+    q, k_new, v_new, tree, scale as for `tree_attention`, lse as it returned it.
+    accepted: int32 [B, A], the accepted drafts of each sequence in their order
+    (the path from the tree's root), negative entries none, A at most 128.
+    positions: int32 [B, T], the drafts' places in their sequences.
+
+    With n accepted drafts, every token's weight becomes
+      mass = exp(-recency_decay * n) * mass + norm * sum_{i,heads} w_i * p_i,
+      w_i = exp(-recency_decay * (n - 1 - i)),
+    p_i the attention probability that accepted draft i gives it (norm 1 if the
+    cache has no norms): `prefill`'s importance, continued over the new tokens.
+    The appended tokens' weights are those that the accepted drafts give them.
+    Rows that do not fit are dropped and reported as `check_status` describes.
+
+    out: a KVCache of the same k and v with bookkeeping of its own, which then
+    receives the new mass, norms, positions and lengths (slots below the new
+    lengths only) while `cache` keeps the old ones.  Default: in place.
+    """
+    out = _check_out(cache, out)
+    tree, tree_stride, scale = _check_drafts(q, k_new, v_new, cache, tree, scale)
+    b, hq, t, _ = q.shape
+    device = cache.k.device
+    if lse.shape != (b, hq, t) or lse.dtype != torch.float32 or lse.device != device:
+        raise ValueError("lse must be FP32 [batch, q_heads, drafts] on the cache's device")
+    if accepted.ndim != 2 or accepted.shape[0] != b or not 1 <= accepted.shape[1] <= MAX_DRAFTS or accepted.dtype != torch.int32 \
+            or accepted.device != device:
+        raise ValueError(f"accepted must be int32 [batch, 1..{MAX_DRAFTS}] on the cache's device")
+    if positions.shape != (b, t) or positions.dtype != torch.int32 or positions.device != device:
+        raise ValueError("positions must be int32 [batch, drafts] on the cache's device")
+    recency_decay = float(recency_decay)
+    if not math.isfinite(recency_decay) or recency_decay < 0:
+        raise ValueError("recency_decay must be finite and nonnegative")
+    lib = _lib.load()
+    size = lib.fe_commit_workspace_bytes(cache._ref, t)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    k_new, v_new = _tma_view(k_new), _tma_view(v_new)
+    lse, accepted, positions = lse.contiguous(), accepted.contiguous(), positions.contiguous()
+    _call(lib.fe_commit_tokens, cache._device_index, cache._ref, out._ref, q.data_ptr(), _strides(q), k_new.data_ptr(),
+          _strides(k_new), v_new.data_ptr(), _strides(v_new), None if tree is None else tree.data_ptr(), tree_stride,
+          lse.data_ptr(), accepted.data_ptr(), accepted.shape[1], positions.data_ptr(), workspace.data_ptr(), size, hq, t,
+          scale, recency_decay)
+    return out
+
+
+def evict_tokens(cache, budget, *, recent=0, out=None):
+    """Cut every row of more than `budget` tokens back to `budget`; returns the cache with the updated bookkeeping.
+
+    Kept are the tokens whose position lies within `recent` of the row's newest,
+    then those of the largest mass (NaN above every number, ties by lower slot).
+    K/V rows move in place: kept tokens below slot `budget` stay, the i-th evicted
+    slot there takes the i-th kept token from above, so a step that is one token
+    over moves one row and the slots' order is not the tokens'.  `out` as for
+    `commit_tokens`, but k and v change all the same.
+    """
+    out = _check_out(cache, out)
+    if isinstance(budget, bool) or not isinstance(budget, int) or budget < 1:
+        raise ValueError("budget must be a positive integer")
+    if isinstance(recent, bool) or not isinstance(recent, int) or not 0 <= recent <= budget:
+        raise ValueError("recent must be an integer in [0, budget]")
+    lib = _lib.load()
+    size = lib.fe_evict_workspace_bytes(cache._ref, budget)
+    workspace = torch.empty(size, dtype=torch.uint8, device=cache.k.device)
+    _call(lib.fe_evict_tokens, cache._device_index, cache._ref, out._ref, budget, recent, workspace.data_ptr(), size)
+    return out

@@ -60,6 +60,7 @@ extern "C" {
 #define FE_STATUS_CUDA 3        /* a CUDA runtime/driver call failed            */
 #define FE_STATUS_TIMEOUT 4     /* a device wait exceeded the watchdog limit    */
 #define FE_STATUS_BAD_INDEX 5   /* a gather index was outside [0, tokens)       */
+#define FE_STATUS_CACHE_FULL 6  /* accepted tokens did not fit in a cache       */
 
 #define FE_DTYPE_F16 0
 #define FE_DTYPE_BF16 1
@@ -288,6 +289,43 @@ FE_API int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t
                              const int64_t* k_new_strides, const void* v_new, const int64_t* v_new_strides,
                              const uint8_t* tree, int64_t tree_batch_stride, void* out, float* lse, void* workspace,
                              int64_t workspace_bytes, int64_t q_heads, int64_t drafts, float scale, void* stream);
+
+/* Adds accepted drafts to a cache: their attention weight to every cached
+ * token, and their K/V rows behind it.
+ * accepted: int32 [batch, max_accepted], the accepted drafts of each sequence in
+ * their order, negative entries none (1 <= max_accepted <= 128; an entry of
+ * `drafts` or more is skipped and raises FE_STATUS_BAD_INDEX).  lse, tree, q,
+ * k_new, scale: as given to and returned by fe_tree_attention.  With n accepted
+ * drafts a_0..a_{n-1} and w_i = exp(-recency_decay * (n-1-i)):
+ *   mass_k = exp(-recency_decay * n) * mass_k
+ *            + norm_k * sum_{i, heads g} w_i * exp(scale * q_{g,a_i}.k - lse_{g,a_i})
+ * (norm_k = 1 without norms), the same sum over the accepted drafts that see it
+ * for each appended token.  Appended slots get their row's norm and
+ * new_positions[b*drafts + a_i]; lengths grow by n, up to the capacity (rows past
+ * it are dropped and raise FE_STATUS_CACHE_FULL).
+ * `out` receives the updated bookkeeping: `cache` itself, or a cache of the same
+ * k and v whose arrays are all others (then `cache` still describes the tokens
+ * before the call); only slots below the new lengths are written.  Each element
+ * is written once in a fixed order (no atomics, bitwise reproducible). */
+FE_API int64_t fe_commit_workspace_bytes(const fe_cache* cache, int64_t drafts);
+FE_API int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, const int64_t* q_strides,
+                            const void* k_new, const int64_t* k_new_strides, const void* v_new,
+                            const int64_t* v_new_strides, const uint8_t* tree, int64_t tree_batch_stride,
+                            const float* lse, const int32_t* accepted, int64_t max_accepted,
+                            const int32_t* new_positions, void* workspace, int64_t workspace_bytes, int64_t q_heads,
+                            int64_t drafts, float scale, float recency_decay, void* stream);
+
+/* Cuts every row of more than `budget` tokens down to `budget`, in place.  The
+ * kept tokens are those whose position is above the row's largest position minus
+ * `recent` (0 <= recent <= budget), then those of the largest mass (NaN above
+ * every number, equal masses by lower slot).  Kept tokens in slots below the
+ * budget stay there; the i-th evicted slot below it takes the i-th kept token at
+ * or above it, so the slots' order changes and only those rows move.  Rows of at
+ * most `budget` tokens are left alone.  `out` as for fe_commit_tokens (k and v
+ * are changed in place all the same).  workspace: fe_evict_workspace_bytes(). */
+FE_API int64_t fe_evict_workspace_bytes(const fe_cache* cache, int64_t budget);
+FE_API int fe_evict_tokens(const fe_cache* cache, const fe_cache* out, int64_t budget, int64_t recent, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 /* Read (and optionally clear) the device status word of `device`: the largest
  * FE_STATUS_* code any kernel raised since the last clear.  Synchronizes that
