@@ -198,9 +198,9 @@ int enter(const void* ptr, void* stream, int* dev_out = nullptr) {
 int padded_dim(int64_t d) { return d <= 64 ? 64 : (d <= 128 ? 128 : (d <= 256 ? 256 : 0)); }
 
 // TMA map over a [B, H, N, D] view with element strides s[4] (s[3] == 1),
-// box = 64 channels x box_rows tokens, 128-byte swizzle, zero fill out of bounds.
+// box = 64 channels x box_rows tokens x box_heads heads, 128-byte swizzle, zero fill out of bounds.
 int make_map(CUtensorMap* m, const void* ptr, const int64_t* s, int64_t B, int64_t H, int64_t N, int64_t D,
-             int dtype, const char* name, int box_rows = 128) {
+             int dtype, const char* name, int box_rows = 128, int box_heads = 1) {
   if (s[3] != 1) return fail(FE_STATUS_UNSUPPORTED, "%s: channel stride must be 1 (got %lld)", name, (long long)s[3]);
   if (reinterpret_cast<uintptr_t>(ptr) % 16)
     return fail(FE_STATUS_UNSUPPORTED, "%s: base pointer must be 16-byte aligned", name);
@@ -222,7 +222,7 @@ int make_map(CUtensorMap* m, const void* ptr, const int64_t* s, int64_t B, int64
     fallback = bytes * ext[i];
   }
   if (box_rows < 1 || box_rows > 256) return fail(FE_STATUS_INVALID, "%s: bad TMA box", name);
-  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_heads, 1};
   cuuint32_t es[4] = {1, 1, 1, 1};
   auto enc = encode_fn();
   if (!enc) return fail(FE_STATUS_CUDA, "cuTensorMapEncodeTiled unavailable");

@@ -54,7 +54,7 @@ int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 // Geometry of a tree-attention launch: a function of the shapes alone, so the
 // workspace query and the launch agree.
 struct TreeGeometry {
-  int rows, parts;  // query rows per work item, partials per run
+  int heads, tile_rows, rows;  // query heads and rows per tile, rows per work item
   bool dual;
   int64_t M, MT, R, D4, ctas, slots, off_stats, off_acc, bytes;
 };
@@ -62,10 +62,12 @@ struct TreeGeometry {
 int tree_geometry(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t drafts, int64_t capacity,
                   int64_t channels, int sms, TreeGeometry* g) {
   const int64_t nbh = batch * kv_heads;
-  g->M = q_heads / kv_heads * drafts;
-  g->dual = channels <= 128 && g->M > 128;
-  g->rows = g->dual ? 256 : 128;
-  g->parts = (channels <= 128 && !g->dual) ? 2 : 1;
+  const int64_t group = q_heads / kv_heads;
+  g->M = group * drafts;
+  g->heads = (int)std::min<int64_t>(group, 128 / drafts);
+  g->tile_rows = g->heads * (int)drafts;
+  g->dual = channels <= 128 && group > g->heads;
+  g->rows = (g->dual ? 2 : 1) * g->tile_rows;
   g->MT = (g->M + g->rows - 1) / g->rows;
   g->R = std::min<int64_t>(g->M, g->rows);
   g->D4 = round_up(channels, 4);
@@ -74,8 +76,8 @@ int tree_geometry(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t draf
   g->ctas = std::min<int64_t>(sms, nbh * g->MT * tiles);
   g->slots = nbh * g->MT + g->ctas;
   g->off_stats = round_up((nbh + 1) * 4, 256);
-  g->off_acc = g->off_stats + round_up(g->slots * g->parts * g->R * 8, 256);
-  g->bytes = g->off_acc + g->slots * g->parts * g->R * g->D4 * 4;
+  g->off_acc = g->off_stats + round_up(g->slots * g->R * 8, 256);
+  g->bytes = g->off_acc + g->slots * g->R * g->D4 * 4;
   return FE_STATUS_OK;
 }
 
@@ -97,7 +99,7 @@ int launch_dependent(Kern kern, dim3 grid, dim3 block, cudaStream_t stream, cons
 }
 
 template <bool BF16, int DP, bool DUAL>
-int launch_tree(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn, const CUtensorMap& tvn,
+int launch_tree(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn, const CUtensorMap& tvn,
                 const fe::TreeParams& p, cudaStream_t stream) {
   using C = fe::TreeCfg<DP, DUAL>;
   auto kern = fe::fe_tree_kernel<BF16, DP, DUAL>;
@@ -116,21 +118,26 @@ int launch_tree(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap&
   if (regs < fe::FWD_REGS_NEEDED)
     return fail(FE_STATUS_UNSUPPORTED, "tree attention kernel compiled with %d registers/thread, needs %d", regs,
                 fe::FWD_REGS_NEEDED);
-  kern<<<dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, stream>>>(tk, tv, tkn, tvn, p);
+  kern<<<dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, stream>>>(tq, tk, tv, tkn, tvn, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
-  const int64_t rows = (int64_t)p.B * p.Hkv * p.M;
-  constexpr int per_cta = fe::TREE_JOIN_THREADS / 32;
-  return launch_dependent(fe::fe_tree_join_kernel<BF16>, dim3((unsigned)((rows + per_cta - 1) / per_cta)),
-                          dim3(fe::TREE_JOIN_THREADS), stream, "tree join launch", p, C::PARTS, C::ROWS);
+  // Warps that share a row's partials: with about `ctas / items` runs a row, one
+  // per two partials, up to the block's eight.
+  const int64_t items = (int64_t)p.B * p.Hkv * p.MT;
+  int splits = 1;
+  while (splits < fe::TREE_JOIN_WARPS && splits * 2 * items < p.nctas) splits *= 2;
+  const int64_t groups = (p.D4 / 4 + fe::TREE_JOIN_QUADS - 1) / fe::TREE_JOIN_QUADS;
+  const int64_t pairs = p.R * groups, per_block = 32 * (fe::TREE_JOIN_WARPS / splits);
+  return launch_dependent(fe::fe_tree_join_kernel<BF16>, dim3((unsigned)items, (unsigned)((pairs + per_block - 1) / per_block)),
+                          dim3(fe::TREE_JOIN_THREADS), stream, "tree join launch", p, C::QTILES * p.tile_rows, splits);
 }
 
 template <bool BF16>
-int launch_tree_dim(int dp, bool dual, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn,
+int launch_tree_dim(int dp, bool dual, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn,
                     const CUtensorMap& tvn, const fe::TreeParams& p, cudaStream_t s) {
-  if (dp == 64) return dual ? launch_tree<BF16, 64, true>(tk, tv, tkn, tvn, p, s) : launch_tree<BF16, 64, false>(tk, tv, tkn, tvn, p, s);
-  if (dp == 128) return dual ? launch_tree<BF16, 128, true>(tk, tv, tkn, tvn, p, s) : launch_tree<BF16, 128, false>(tk, tv, tkn, tvn, p, s);
-  return launch_tree<BF16, 256, false>(tk, tv, tkn, tvn, p, s);
+  if (dp == 64) return dual ? launch_tree<BF16, 64, true>(tq, tk, tv, tkn, tvn, p, s) : launch_tree<BF16, 64, false>(tq, tk, tv, tkn, tvn, p, s);
+  if (dp == 128) return dual ? launch_tree<BF16, 128, true>(tq, tk, tv, tkn, tvn, p, s) : launch_tree<BF16, 128, false>(tq, tk, tv, tkn, tvn, p, s);
+  return launch_tree<BF16, 256, false>(tq, tk, tv, tkn, tvn, p, s);
 }
 
 }  // namespace
@@ -170,7 +177,8 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   if ((rc = tree_geometry(B, q_heads, H, drafts, cache->capacity, D, sm_count(dev), &g))) return rc;
   if (workspace_bytes < g.bytes)
     return fail(FE_STATUS_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)g.bytes);
-  CUtensorMap tk, tv, tkn, tvn;
+  CUtensorMap tq, tk, tv, tkn, tvn;
+  if ((rc = make_map(&tq, q, q_strides, B, q_heads, drafts, D, cache->dtype, "q", (int)drafts, g.heads))) return rc;
   if ((rc = make_map(&tk, cache->k, cache->k_strides, B, H, cache->capacity, D, cache->dtype, "cache k"))) return rc;
   if ((rc = make_map(&tv, cache->v, cache->v_strides, B, H, cache->capacity, D, cache->dtype, "cache v"))) return rc;
   if ((rc = make_map(&tkn, k_new, k_new_strides, B, H, drafts, D, cache->dtype, "k_new"))) return rc;
@@ -190,7 +198,7 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.base = reinterpret_cast<int32_t*>(ws);
   p.stats = reinterpret_cast<float2*>(ws + g.off_stats);
-  p.acc = reinterpret_cast<float*>(ws + g.off_acc);
+  p.acc = reinterpret_cast<float4*>(ws + g.off_acc);
   p.B = (int)B;
   p.Hq = (int)q_heads;
   p.Hkv = (int)H;
@@ -199,17 +207,18 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   p.D = (int)D;
   p.capacity = (int)cache->capacity;
   p.M = (int)g.M;
+  p.tile_rows = g.tile_rows;
   p.MT = (int)g.MT;
   p.R = (int)g.R;
   p.D4 = (int)g.D4;
   p.nctas = (int)g.ctas;
   p.sc = (float)((double)scale * 1.4426950408889634);
-  p.q_vec = rows_are_vectors(q, q_strides, B, q_heads, drafts, D) ? 1 : 0;
+  p.tree_vec = tree && drafts % 16 == 0 && reinterpret_cast<uintptr_t>(tree) % 16 == 0 && tree_batch_stride % 16 == 0;
   p.timeout_ns = (uint64_t)g_watchdog_ns;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int dp = padded_dim(D);
-  return cache->dtype == FE_DTYPE_BF16 ? launch_tree_dim<true>(dp, g.dual, tk, tv, tkn, tvn, p, s)
-                                       : launch_tree_dim<false>(dp, g.dual, tk, tv, tkn, tvn, p, s);
+  return cache->dtype == FE_DTYPE_BF16 ? launch_tree_dim<true>(dp, g.dual, tq, tk, tv, tkn, tvn, p, s)
+                                       : launch_tree_dim<false>(dp, g.dual, tq, tk, tv, tkn, tvn, p, s);
 }
 
 }  // extern "C"

@@ -6,8 +6,8 @@
 //   lse = log sum exp s   (out 0 and lse -inf for a row that sees nothing).
 //
 // The G query heads of a KV head share its keys, so the G*T queries of one
-// (b, hkv) are the rows of one matrix product: row r = g*T + t, tiles of 128
-// rows on the TMEM lanes.  What bounds it is reading K and V once (4*D bytes a
+// (b, hkv) are the rows of one matrix product: row g*T + t, in tiles of as many
+// whole heads as fit the 128 TMEM lanes (one TMA box {64 channels, T, heads}).  What bounds it is reading K and V once (4*D bytes a
 // cached token) until G*T reaches about 250 rows, then the tensor pipe; the
 // padding of few rows to a 128-row MMA costs nothing that the memory time does
 // not cover (1024 tensor cycles a tile against ~2800 cycles of HBM time an SM).
@@ -43,12 +43,14 @@ struct TreeParams {
   uint16_t* out;  // [B, Hq, T, D] contiguous
   float* lse;     // [B, Hq, T]
   int32_t* base;  // workspace: first unit of every row, total
-  float2* stats;  // workspace: [slots][groups][R] {m, l}
-  float* acc;     // workspace: [slots][groups][R][D4]
+  float2* stats;  // workspace: [slots][R] {m, l}
+  float4* acc;    // workspace: [slots][D4/4][R]: consecutive rows are consecutive in memory
   int B, Hq, Hkv, G, T, D, capacity;
-  int M, MT, R, D4, nctas;
+  int M;             // G*T query rows of a KV head
+  int tile_rows;     // of them in a 128-row tile: whole heads
+  int MT, R, D4, nctas;
   float sc;  // scale * log2(e)
-  int q_vec;
+  int tree_vec;      // mask rows can be read 16 bytes at a time
   uint64_t timeout_ns;
 };
 
@@ -56,8 +58,7 @@ template <int DP, bool DUAL>
 struct TreeCfg {
   static_assert(!DUAL || DP <= 128, "two query tiles need two O accumulators");
   static constexpr int NG = DP <= 128 ? 2 : 1;       // softmax warpgroups
-  static constexpr int ROWS = DUAL ? 256 : 128;      // query rows per work item
-  static constexpr int PARTS = (NG == 2 && !DUAL) ? 2 : 1;  // partials a run leaves per row
+  static constexpr bool SPLIT = NG == 2 && !DUAL;
   static constexpr int TILE = 128 * DP * 2;          // bytes of a 128-row tile
   static constexpr int NCH = DP / 64;
   static constexpr int QTILES = DUAL ? 2 : 1;
@@ -66,10 +67,11 @@ struct TreeCfg {
   static constexpr int OFF_K = QTILES * TILE;
   static constexpr int OFF_V = OFF_K + STAGES * TILE;
   static constexpr int OFF_BAR = OFF_V + STAGES * TILE;
-  // q_full, k_full[S], v_full[S], k_empty[S], v_empty[S], s_full[2], p_full[2], o_full[2], drain
-  static constexpr int NBAR = 1 + 4 * STAGES + 7;
+  // q_full[2], q_empty[2], k_full[S], v_full[S], k_empty[S], v_empty[S], s_full[2], p_full[2], o_full[2], drain
+  static constexpr int NBAR = 4 + 4 * STAGES + 7;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
-  static constexpr int SMEM = OFF_MISC + 16 + 32 + DEC_SCRATCH_INTS * 4 + 1024;
+  static constexpr int OFF_ML = OFF_MISC + 16 + 64 + DEC_SCRATCH_INTS * 4;  // float2[128]
+  static constexpr int SMEM = OFF_ML + (SPLIT ? 128 * 8 : 0) + 1024;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int THREADS = 384;
 };
@@ -77,22 +79,19 @@ struct TreeCfg {
 // Lowest running max: finite, so that a row which has seen no key yet rescales
 // by 2^-huge = 0 and never forms inf - inf.
 constexpr float TREE_M0 = -3.0e38f;
+constexpr uint32_t TREE_QBUF = 8192;  // bytes between the halves of a query tile's 64-column group
 
-// One key tile of a row's softmax (S in x).  KIND 0: every column counts;
-// 1: columns past lim do not; 2: only columns with their bit set do.
-template <bool BF16, int DV, int KIND>
-__device__ __forceinline__ void tree_softmax_tile(float (&x)[128], bool first, int lim, const uint32_t (&bits)[4],
+// One key tile of a row's softmax (S in x).  With `masked`, only columns with
+// their bit set count.
+template <bool BF16, int DV>
+__device__ __forceinline__ void tree_softmax_tile(float (&x)[128], bool first, bool masked, const uint32_t (&bits)[4],
                                                   float sc, float sce, bool sc_pos, float& m_used, float& l,
                                                   uint32_t tS, uint32_t tO) {
   if (!sc_pos) {
 #pragma unroll
     for (int c = 0; c < 128; ++c) x[c] *= sc;
   }
-  if constexpr (KIND == 1) {
-#pragma unroll
-    for (int c = 0; c < 128; ++c) x[c] = (c <= lim) ? x[c] : -INFINITY;
-  }
-  if constexpr (KIND == 2) {
+  if (masked) {
 #pragma unroll
     for (int c = 0; c < 128; ++c) x[c] = ((bits[c >> 5] >> (c & 31)) & 1u) ? x[c] : -INFINITY;
   }
@@ -141,8 +140,22 @@ __device__ __forceinline__ void tree_bits(const TreeParams& p, int b, int t, uin
   for (int w = 0; w < 4; ++w) {
     const int n = min(max(p.T - 32 * w, 0), 32);
     uint32_t v = 0u;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) v |= (__ldg(row + 32 * w + j) != 0 ? 1u : 0u) << j;
+    if (p.tree_vec) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (16 * u >= n) continue;
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + 32 * w) + u);
+        // Four mask bytes to four bits: 1 where nonzero, gathered by a multiply.
+        v |= ((__vsetgtu4(x.x, 0u) * 0x01020408u) >> 24) << (16 * u);
+        v |= ((__vsetgtu4(x.y, 0u) * 0x01020408u) >> 24) << (16 * u + 4);
+        v |= ((__vsetgtu4(x.z, 0u) * 0x01020408u) >> 24) << (16 * u + 8);
+        v |= ((__vsetgtu4(x.w, 0u) * 0x01020408u) >> 24) << (16 * u + 12);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < n) v |= (__ldg(row + 32 * w + j) != 0 ? 1u : 0u) << j;
+    }
     bits[w] = v;
   }
 }
@@ -152,7 +165,7 @@ __device__ __forceinline__ void tree_bits(const TreeParams& p, int b, int t, uin
 // only rows that see such a draft come here (see the draft tile).
 template <bool BF16>
 __device__ __noinline__ void tree_add_special(const TreeParams& p, int b, int h, int g, int t, uint32_t bits, int j0,
-                                              float m, float* o) {
+                                              float m, float4* o) {
   const uint16_t* q = p.q + b * p.q_sb + (static_cast<int64_t>(h) * p.G + g) * p.q_sh + t * p.q_st;
   for (; bits != 0u; bits &= bits - 1u) {
     const int j = j0 + __ffs(bits) - 1;
@@ -161,7 +174,7 @@ __device__ __noinline__ void tree_add_special(const TreeParams& p, int b, int h,
     float s = 0.f;
     for (int d = 0; d < p.D; ++d) s = fmaf(elem_to_float<BF16>(q[d]), elem_to_float<BF16>(k[d]), s);
     const float w = ex2_approx(s * p.sc - m);
-    for (int c = 0; c < p.D; ++c) o[c] += w * elem_to_float<BF16>(v[c]);
+    for (int c = 0; c < p.D; ++c) reinterpret_cast<float*>(o + (c >> 2) * p.R)[c & 3] += w * elem_to_float<BF16>(v[c]);
   }
 }
 
@@ -173,7 +186,8 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
 
 template <bool BF16, int DP, bool DUAL>
 __global__ void __launch_bounds__(384, 1)
-    fe_tree_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+    fe_tree_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                   const __grid_constant__ CUtensorMap tv,
                    const __grid_constant__ CUtensorMap tkn, const __grid_constant__ CUtensorMap tvn,
                    const __grid_constant__ TreeParams p) {
   using C = TreeCfg<DP, DUAL>;
@@ -181,7 +195,8 @@ __global__ void __launch_bounds__(384, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* k_full = q_full + 1;
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* k_full = q_empty + 2;
   uint64_t* v_full = k_full + C::STAGES;
   uint64_t* k_empty = v_full + C::STAGES;
   uint64_t* v_empty = k_empty + C::STAGES;
@@ -191,17 +206,29 @@ __global__ void __launch_bounds__(384, 1)
   uint64_t* drain = o_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  // Drafts whose V row is not finite, 128 bits, one set per segment parity.
+  // Drafts whose V row is not finite, 128 bits: [group that took the draft tile][segment parity].
   uint32_t* special = tmem_holder + 4;
-  int* scratch = reinterpret_cast<int*>(special + 8);
+  int* scratch = reinterpret_cast<int*>(special + 16);
+
+  float2* s_ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
+  if (threadIdx.x == 256) {
+    tma_prefetch_desc(&tq);
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+    tma_prefetch_desc(&tkn);
+    tma_prefetch_desc(&tvn);
+  }
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    mbar_init(q_full, 4 * NG);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&v_full[s], 1);
@@ -228,6 +255,11 @@ __global__ void __launch_bounds__(384, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const uint64_t TO = p.timeout_ns;
+  // Query tiles of at most 64 rows are double-buffered in the two halves of
+  // the tile, so a run's next row starts while the last one is written out.  The
+  // MMA reads 128 rows all the same: the others' scores stay on their own TMEM
+  // lanes, which nobody reads.
+  const uint32_t qbufs = !DUAL && p.tile_rows <= 64 ? 2 : 1;
   DecSegment sg;
 
   if (warp >= 8) {
@@ -235,16 +267,24 @@ __global__ void __launch_bounds__(384, 1)
     if (warp == 8) {
       // ---------------------------------------------------------- producer --
       if (lane == 0) {
-        tma_prefetch_desc(&tk);
-        tma_prefetch_desc(&tv);
-        tma_prefetch_desc(&tkn);
-        tma_prefetch_desc(&tvn);
         uint32_t loads[C::STAGES];
         for (int s = 0; s < C::STAGES; ++s) loads[s] = 0;
         bool ok = true;
-        uint32_t it = 0;
+        uint32_t it = 0, nseg = 0;
+        const int heads = p.tile_rows / p.T;  // per query tile
         while (ok && walk.next(sg)) {
           const int b = sg.bh / p.Hkv, h = sg.bh - b * p.Hkv;
+          // The segment's queries: whole heads, their rows one after another.
+          // (Rows past the last head of the KV head are read and not used.)
+          const uint32_t qb = nseg % qbufs, quse = nseg / qbufs;
+          if (quse > 0) ok = mbar_wait(&q_empty[qb], (quse - 1) & 1, TO, abort_flag);
+          if (!ok) break;
+          mbar_expect_tx(&q_full[qb], C::QTILES * p.tile_rows * DP * 2);
+          for (int t = 0; t < C::QTILES; ++t)
+            for (int c = 0; c < C::NCH; ++c)
+              tma_load_4d(smem + C::OFF_Q + t * C::TILE + c * 16384 + qb * TREE_QBUF, &tq, &q_full[qb], c * 64, 0,
+                          h * p.G + (sg.mt * C::QTILES + t) * heads, b);
+          ++nseg;
           for (int j = sg.j0; j < sg.j1; ++j, ++it) {
             const int s = it % C::STAGES;
             const uint32_t use = it / C::STAGES;
@@ -269,6 +309,8 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
         // Never leave the CTA with a TMA write in flight.
+        for (uint32_t i = nseg > qbufs ? nseg - qbufs : 0; i < nseg; ++i)
+          mbar_wait_inflight(&q_full[i % qbufs], (i / qbufs) & 1, TO);
         for (int s = 0; s < C::STAGES; ++s) {
           if (loads[s] == 0) continue;
           const uint32_t use = (loads[s] - 1) / 2;
@@ -298,6 +340,7 @@ __global__ void __launch_bounds__(384, 1)
         while (ok && walk.next(sg)) {
           const int ntile = sg.j1 - sg.j0;
           const int steps = DUAL ? 2 * ntile : ntile;
+          const uint32_t qb = nseg % qbufs;
           auto tile_of = [&](int i) { return it0 + static_cast<uint32_t>(DUAL ? i >> 1 : i); };
           auto issue_s = [&](int i) -> bool {
             const uint32_t tile = tile_of(i);
@@ -306,7 +349,7 @@ __global__ void __launch_bounds__(384, 1)
               if (!mbar_wait(&k_full[s], (tile / C::STAGES) & 1, TO, abort_flag)) return false;
               tc_fence_after();
             }
-            const uint32_t a = dq_lo + (DUAL ? t * TILE16 : 0u);
+            const uint32_t a = dq_lo + (DUAL ? t * TILE16 : qb * (TREE_QBUF >> 4));
             const uint32_t bb = dk_lo + s * TILE16;
 #pragma unroll 8
             for (int kk = 0; kk < DP / 16; ++kk) {
@@ -315,9 +358,10 @@ __global__ void __launch_bounds__(384, 1)
             }
             umma_commit(&s_full[t]);
             if (!DUAL || (i & 1) == 1) umma_commit(&k_empty[s]);
+            if (i == steps - 1) umma_commit(&q_empty[qb]);
             return true;
           };
-          ok = mbar_wait(q_full, nseg & 1, TO, abort_flag);
+          ok = mbar_wait(&q_full[qb], (nseg / qbufs) & 1, TO, abort_flag);
           if (!ok) break;
           tc_fence_after();
           for (int i = 0; i < NG && i < steps && ok; ++i) ok = issue_s(i);
@@ -338,9 +382,7 @@ __global__ void __launch_bounds__(384, 1)
             if (i + NG < steps) ok = issue_s(i + NG);
             else umma_commit(&o_full[t]);
           }
-          // A group without a step still learns that the segment's products
-          // are done (it rewrites its share of the query tile next).
-          if (ok && steps < NG) umma_commit(&o_full[1]);
+          if (ok && steps < NG) umma_commit(&o_full[1]);  // one commit a segment for a group without a step, too
           it0 += ntile;
           ++nseg;
         }
@@ -364,48 +406,29 @@ __global__ void __launch_bounds__(384, 1)
       uint32_t it0 = 0, nseg = 0, ns = 0;  // key tiles before, segments, S tiles of this group
       for (; walk.next(sg); ++nseg) {
         const int b = sg.bh / p.Hkv, h = sg.bh - b * p.Hkv;
-        const int row = sg.mt * C::ROWS + (DUAL ? t * 128 : 0) + r;  // of the item's G*T queries
-        const bool live = row < p.M;
-        const bool warp_live = row - static_cast<int>(lane) < p.M;
+        const int ntile = sg.j1 - sg.j0;
+        const int pr = (DUAL ? t * p.tile_rows : 0) + r;  // row of the item
+        const int row = sg.mt * C::QTILES * p.tile_rows + pr;  // of the KV head's G*T queries
+        const bool live = r < p.tile_rows && row < p.M;
+        const bool warp_live = __any_sync(0xffffffffu, live);
         const int g = live ? row / p.T : 0, tt = live ? row - g * p.T : 0;
-        uint32_t* spec = special + (nseg & 1) * 4;
-        // ---- query tile into shared memory (padding rows and channels zero)
-        {
-          const int rows0 = DUAL ? t * 128 : t * (128 / NG);
-          const int nrows = DUAL ? 128 : 128 / NG;
-          constexpr int CPR = DP / 8;
-          const int tid = r;
-          const uint16_t* qb = p.q + b * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
-          for (int i0 = tid; i0 < nrows * CPR; i0 += 128 * 4) {
-            uint4 v[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int i = i0 + u * 128;
-              v[u] = make_uint4(0u, 0u, 0u, 0u);
-              const int qr = sg.mt * C::ROWS + rows0 + i / CPR;
-              if (i < nrows * CPR && qr < p.M) {
-                const int qg = qr / p.T;
-                v[u] = load_row_chunk(qb + qg * p.q_sh + (qr - qg * p.T) * p.q_st, i % CPR, p.D, p.q_vec);
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int i = i0 + u * 128;
-              if (i < nrows * CPR) {
-                const int lr = rows0 + i / CPR;
-                *reinterpret_cast<uint4*>(smem + C::OFF_Q + (lr >> 7) * C::TILE +
-                                          sw128_offset(lr & 127, i % CPR, 16384)) = v[u];
-              }
-            }
+        // Who takes the draft tile notes which drafts its rows see, and starts a
+        // clean list of drafts that need special care.
+        const bool has_drafts = sg.j1 == sg.tiles;
+        const int owner = DUAL ? 0 : (ntile - 1) % NG;  // group that takes the last tile (DUAL: that clears its V rows)
+        const bool mine = has_drafts && (DUAL || owner == t);
+        uint32_t* spec = special + owner * 8 + (nseg & 1) * 4;
+        uint32_t bits[4] = {0u, 0u, 0u, 0u};
+        if (mine) {
+          if (live) tree_bits(p, b, tt, bits);
+          if (t == owner) {
+            named_bar_sync(1 + t, 128);
+            if (r < 4) spec[r] = 0u;
+            named_bar_sync(1 + t, 128);
           }
-          if (t == 0 && r < 4) spec[r] = 0u;
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(q_full);
         }
         float m_used = TREE_M0, l = 0.f;
         bool first = true;
-        const int ntile = sg.j1 - sg.j0;
         for (int i = DUAL ? 0 : t; i < ntile && ok; i += DUAL ? 1 : NG) {
           const int j = sg.j0 + i;
           const uint32_t tile = it0 + i;
@@ -451,15 +474,17 @@ __global__ void __launch_bounds__(384, 1)
               tmem_ld64_sync(tS, xr);
               tmem_ld64_sync(tS + 64, xr + 64);
             }
-            uint32_t bits[4] = {0u, 0u, 0u, 0u};
-            if (drafts) {
-              if (live) tree_bits(p, b, tt, bits);
-              tree_softmax_tile<BF16, DP, 2>(x, first, lim, bits, sc, sce, sc_pos, m_used, l, tS, tO);
-            } else if (lim < 127) {
-              tree_softmax_tile<BF16, DP, 1>(x, first, lim, bits, sc, sce, sc_pos, m_used, l, tS, tO);
-            } else {
-              tree_softmax_tile<BF16, DP, 0>(x, first, lim, bits, sc, sce, sc_pos, m_used, l, tS, tO);
+            uint32_t sees[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int n = min(max(lim + 1 - 32 * w, 0), 32);
+              sees[w] = drafts ? bits[w] : (n == 32 ? 0xffffffffu : ((1u << n) - 1u));
             }
+            const bool masked = drafts || lim < 127;
+            if (DUAL && !masked)  // the long runs' loop, free of masking code
+              tree_softmax_tile<BF16, DP>(x, first, false, sees, sc, sce, sc_pos, m_used, l, tS, tO);
+            else
+              tree_softmax_tile<BF16, DP>(x, first, masked, sees, sc, sce, sc_pos, m_used, l, tS, tO);
           }
           first = false;
           tc_fence_before();
@@ -468,34 +493,92 @@ __global__ void __launch_bounds__(384, 1)
         }
         if (ok) ok = warp_all(mbar_wait(&o_full[t], nseg & 1, TO, abort_flag));
         tc_fence_after();
-        // ---- partial result of this run for the row
-        const int64_t slot = (static_cast<int64_t>(sg.bh) * p.MT + sg.mt + blockIdx.x) * C::PARTS + (DUAL ? 0 : t);
-        const int pr = (DUAL ? t * 128 : 0) + r;
+        // ---- result of this run for the row: a partial, or the row itself
+        // when the run has all of its tiles
+        const bool whole = sg.j0 == 0 && sg.j1 == sg.tiles;
         const float nan = __int_as_float(0x7fffffff);
-        if (live) p.stats[slot * p.R + pr] = ok ? make_float2(m_used, l) : make_float2(nan, nan);
-        if (ok && !first && warp_live) {
-          float* dst = p.acc + (slot * p.R + pr) * p.D4;
+        float f0 = 1.f, f1 = 0.f;  // weights of O of this group's lanes, and (SPLIT) of the other warpgroup's
+        if (!ok) m_used = l = nan;  // aborted (watchdog): everything below becomes NaN
+        if constexpr (C::SPLIT) {
+          // Both warpgroups hold the row (lane r of two O tiles); each writes
+          // half of the channels of their sum.
+          const float2 own = make_float2(m_used, l);
+          if (t == 1) s_ml[r] = own;
+          named_bar_sync(3, 256);
+          float2 a = own, c = own;
+          if (t == 0) {
+            c = s_ml[r];
+            s_ml[r] = own;
+          }
+          named_bar_sync(3, 256);
+          if (t == 1) a = s_ml[r];
+          m_used = fmaxf(a.x, c.x);
+          f0 = ex2_approx(a.x - m_used);
+          f1 = ex2_approx(c.x - m_used);
+          l = a.y * f0 + c.y * f1;
+        }
+        const bool two = C::SPLIT && ntile > 1;
+        const int64_t slot = static_cast<int64_t>(sg.bh) * p.MT + sg.mt + blockIdx.x;
+        const int64_t orow = static_cast<int64_t>(sg.bh) * p.M + row;
+        float4* dst = p.acc + slot * p.R * (p.D4 / 4) + pr;
+        uint16_t* out = p.out + orow * p.D;
+        // Special rows are added in memory, so such a run's sum goes through it.
+        const bool special_rows = has_drafts && (spec[0] | spec[1] | spec[2] | spec[3]) != 0u;
+        const bool direct = whole && !special_rows;
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        if (live && (!C::SPLIT || t == 0)) {
+          if (whole) p.lse[orow] = l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
+          else p.stats[slot * p.R + pr] = make_float2(m_used, l);
+        }
+        if (warp_live) {
+          constexpr int CB = C::SPLIT ? DP / 2 : DP;
 #pragma unroll 1
-          for (int c0 = 0; c0 < DP; c0 += 32) {
+          for (int c0 = C::SPLIT ? t * CB : 0; c0 < (C::SPLIT ? (t + 1) * CB : DP); c0 += 32) {
             uint32_t o[32];
-            tmem_ld32_sync(tO + c0, o);
-            if (live) {
+            tmem_ld32_sync((C::SPLIT ? tO - t * DP : tO) + c0, o);
+            if (two) {
+              uint32_t o1[32];
+              tmem_ld32_sync(tO - t * DP + DP + c0, o1);
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                o[c] = __float_as_uint(__uint_as_float(o[c]) * f0 + __uint_as_float(o1[c]) * f1);
+            }
+            if (live && direct) {
+#pragma unroll
+              for (int c = 0; c < 32; c += 8) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  w[e] = pack2<BF16>(__uint_as_float(o[c + 2 * e]) * inv, __uint_as_float(o[c + 2 * e + 1]) * inv);
+                if ((p.D & 7) == 0) {
+                  if (c0 + c < p.D) *reinterpret_cast<uint4*>(out + c0 + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e)
+                    if (c0 + c + e < p.D) out[c0 + c + e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+                }
+              }
+            } else if (live) {
 #pragma unroll
               for (int q4 = 0; q4 < 8; ++q4)
                 if (c0 + q4 * 4 < p.D4)
-                  *reinterpret_cast<uint4*>(dst + c0 + q4 * 4) =
+                  *reinterpret_cast<uint4*>(dst + (c0 / 4 + q4) * p.R) =
                       make_uint4(o[4 * q4], o[4 * q4 + 1], o[4 * q4 + 2], o[4 * q4 + 3]);
             }
           }
-          // Only the group that took the draft tile adds its special rows.
-          if ((spec[0] | spec[1] | spec[2] | spec[3]) != 0u && live && (DUAL || (ntile - 1) % NG == t)) {
-            uint32_t bits[4];
-            tree_bits(p, b, tt, bits);
+        }
+        if (special_rows) {
+          if constexpr (C::SPLIT) named_bar_sync(3, 256);
+          if (mine && live) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) tree_add_special<BF16>(p, b, h, g, tt, bits[w] & spec[w], 32 * w, m_used, dst);
+            if (whole)
+              for (int c = 0; c < p.D; ++c)
+                out[c] = static_cast<uint16_t>(pack2<BF16>(reinterpret_cast<float*>(dst + (c >> 2) * p.R)[c & 3] * inv, 0.f));
           }
         }
         tc_fence_before();
+        if constexpr (C::SPLIT) named_bar_sync(3, 256);  // both are done with both O tiles
         it0 += ntile;
       }
     }
@@ -510,86 +593,111 @@ __global__ void __launch_bounds__(384, 1)
   }
 }
 
-constexpr int TREE_JOIN_THREADS = 128;
+constexpr int TREE_JOIN_THREADS = 256;
+constexpr int TREE_JOIN_WARPS = TREE_JOIN_THREADS / 32;
+constexpr int TREE_JOIN_QUADS = 4;  // channel quads per thread
 
-// Joins the runs' partials of one query row (one warp): the rows' weights
-// 2^(m_i - max m) in the order of the runs.
+// Joins the runs' partials of a row.  A thread owns 16 channels of one row
+// (consecutive threads: consecutive rows, as the partials lie) and merges
+// every splits-th partial with a running maximum; the `splits` warps that share
+// a set of rows are merged through shared memory in a fixed order.
 template <bool BF16>
-__global__ void __launch_bounds__(TREE_JOIN_THREADS) fe_tree_join_kernel(const __grid_constant__ TreeParams p, int parts, int rows_per_item) {
+__global__ void __launch_bounds__(TREE_JOIN_THREADS)
+    fe_tree_join_kernel(const __grid_constant__ TreeParams p, int rows_per_item, int splits) {
+  constexpr int Q = TREE_JOIN_QUADS;
+  __shared__ float4 s_acc[TREE_JOIN_WARPS][Q][32];
+  __shared__ float2 s_ml[TREE_JOIN_WARPS][32];
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t orow = static_cast<int64_t>(blockIdx.x) * (TREE_JOIN_THREADS / 32) + (threadIdx.x >> 5);
-  if (orow >= static_cast<int64_t>(p.B) * p.Hkv * p.M) return;
-  const int bh = static_cast<int>(orow / p.M);
-  const int row = static_cast<int>(orow - static_cast<int64_t>(bh) * p.M);
-  const int mt = row / rows_per_item, pr = row - mt * rows_per_item;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int split = warp % splits;
+  const int quads = p.D4 / 4, groups = (quads + Q - 1) / Q;
+  const int item = blockIdx.x;
+  const int bh = item / p.MT, mt = item - bh * p.MT;
+  const int rows = min(p.M - mt * rows_per_item, rows_per_item);
+  const int pair = (blockIdx.y * (TREE_JOIN_WARPS / splits) + warp / splits) * 32 + lane;
+  const bool live = pair < rows * groups;
+  const int quad0 = live ? pair / rows * Q : 0, r = live ? pair % rows : 0;
   const int total = p.base[p.B * p.Hkv];
-  const int per = (total + p.nctas - 1) / p.nctas;
   const int start = p.base[bh];
   const int tiles = (p.base[bh + 1] - start) / p.MT;
+  const int per = (total + p.nctas - 1) / p.nctas;
   const int u0 = start + mt * tiles;
-  const int c0 = u0 / per, c1 = (u0 + tiles - 1) / per;
-  const int64_t slot0 = (static_cast<int64_t>(bh) * p.MT + mt + c0) * parts;
-  const int n = (c1 - c0 + 1) * parts;
-  float m = TREE_M0, bad = 0.f;
-  for (int i = lane; i < n; i += 32) {
-    const float2 st = p.stats[(slot0 + i) * p.R + pr];
-    if (st.y != 0.f) m = fmaxf(m, st.x);
-    bad += st.x * 0.f + st.y * 0.f;  // NaN or inf statistics mark the row
-  }
+  const int c0 = u0 / per, n = (u0 + tiles - 1) / per - c0 + 1;
+  if (n == 1) return;  // one run had the whole row and wrote it
+  const int64_t slot0 = static_cast<int64_t>(item) + c0;
+  const float2* st_row = p.stats + slot0 * p.R + r;
+  const float4* acc_row = p.acc + slot0 * p.R * quads + static_cast<int64_t>(quad0) * p.R + r;
+  const int64_t acc_step = static_cast<int64_t>(p.R) * quads;
+  float m = TREE_M0, l = 0.f;
+  float4 a[Q];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    bad += __shfl_xor_sync(0xffffffffu, bad, o);
-  }
-  // lane holds columns 4*lane .. +3, and the same 128 further on
-  float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  float l = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    float2 st = make_float2(TREE_M0, 0.f);
-    if (i0 + lane < n) st = p.stats[(slot0 + i0 + lane) * p.R + pr];
-    const float w_mine = st.y != 0.f ? exp2f(st.x - m) : 0.f;
-    const float l_mine = st.y;
-    const int k = min(32, n - i0);
-#pragma unroll 4
-    for (int i = 0; i < k; ++i) {
-      const float w = __shfl_sync(0xffffffffu, w_mine, i);
-      const float li = __shfl_sync(0xffffffffu, l_mine, i);
-      if (li == 0.f) continue;  // this run saw no key of the row
-      l = fmaf(w, li, l);
-      const float* src = p.acc + ((slot0 + i0 + i) * p.R + pr) * p.D4;
+  for (int j = 0; j < Q; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto merge = [&](float2 st, const float4 (&v)[Q]) {
+    if (st.y == 0.f) return;  // this run saw no key of the row: its O was not written
+    const float mn = fmaxf(m, st.x);
+    const float f = exp2f(m - mn), g = exp2f(st.x - mn);
+    m = mn;
+    l = l * f + st.y * g;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int c = e * 128 + lane * 4;
-        if (c < p.D4) {
-          const float4 v = *reinterpret_cast<const float4*>(src + c);
-          acc[e][0] = fmaf(w, v.x, acc[e][0]);
-          acc[e][1] = fmaf(w, v.y, acc[e][1]);
-          acc[e][2] = fmaf(w, v.z, acc[e][2]);
-          acc[e][3] = fmaf(w, v.w, acc[e][3]);
+    for (int j = 0; j < Q; ++j) {
+      a[j].x = a[j].x * f + v[j].x * g;
+      a[j].y = a[j].y * f + v[j].y * g;
+      a[j].z = a[j].z * f + v[j].z * g;
+      a[j].w = a[j].w * f + v[j].w * g;
+    }
+  };
+  if (live) {
+    constexpr int U = 3;
+    for (int i0 = split; i0 < n; i0 += splits * U) {
+      float2 st[U];
+      float4 v[U][Q];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * splits;
+        st[u] = make_float2(0.f, 0.f);
+        if (i < n) {
+          st[u] = __ldcs(st_row + static_cast<int64_t>(i) * p.R);
+#pragma unroll
+          for (int j = 0; j < Q; ++j)
+            if (quad0 + j < quads) v[u][j] = __ldcs(acc_row + i * acc_step + j * p.R);
         }
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) merge(st[u], v[u]);
     }
   }
-  l += bad;
+  if (splits > 1) {
+    s_ml[warp][lane] = make_float2(m, l);
+#pragma unroll
+    for (int j = 0; j < Q; ++j) s_acc[warp][j][lane] = a[j];
+    __syncthreads();
+    if (split != 0) return;
+    for (int w = 1; w < splits; ++w) {
+      float4 v[Q];
+#pragma unroll
+      for (int j = 0; j < Q; ++j) v[j] = s_acc[warp + w][j][lane];
+      merge(s_ml[warp + w][lane], v);
+    }
+  }
+  if (!live) return;
   const bool none = l == 0.f;
   const float inv = none ? 0.f : 1.0f / l;
+  const int64_t orow = static_cast<int64_t>(bh) * p.M + mt * rows_per_item + r;
   uint16_t* out = p.out + orow * p.D;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int c = e * 128 + lane * 4;
+  for (int j = 0; j < Q; ++j) {
+    const int c = (quad0 + j) * 4;
     if (c >= p.D) continue;
-    const uint32_t a = pack2<BF16>(acc[e][0] * inv, acc[e][1] * inv);
-    const uint32_t b2 = pack2<BF16>(acc[e][2] * inv, acc[e][3] * inv);
+    const uint32_t lo = pack2<BF16>(a[j].x * inv, a[j].y * inv), hi = pack2<BF16>(a[j].z * inv, a[j].w * inv);
     if ((p.D & 3) == 0) {
-      *reinterpret_cast<uint2*>(out + c) = make_uint2(a, b2);
+      *reinterpret_cast<uint2*>(out + c) = make_uint2(lo, hi);
     } else {
-      const uint16_t w[4] = {static_cast<uint16_t>(a), static_cast<uint16_t>(a >> 16), static_cast<uint16_t>(b2),
-                             static_cast<uint16_t>(b2 >> 16)};
+      const uint16_t w[4] = {static_cast<uint16_t>(lo), static_cast<uint16_t>(lo >> 16), static_cast<uint16_t>(hi),
+                             static_cast<uint16_t>(hi >> 16)};
       for (int i = 0; i < 4 && c + i < p.D; ++i) out[c + i] = w[i];
     }
   }
-  if (lane == 0) p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  if (quad0 == 0) p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
 }
 
 }  // namespace fe

@@ -175,9 +175,7 @@ def tree_attention(q, k_new, v_new, cache, *, tree=None, scale=None):
     out = torch.empty((b, hq, t, d), dtype=q.dtype, device=device)
     lse = torch.empty((b, hq, t), dtype=torch.float32, device=device)
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    k_new, v_new = _tma_view(k_new), _tma_view(v_new)
+    q, k_new, v_new = _tma_view(q), _tma_view(k_new), _tma_view(v_new)
     _call(lib.fe_tree_attention, cache._device_index, cache._ref, q.data_ptr(), _strides(q), k_new.data_ptr(), _strides(k_new),
           v_new.data_ptr(), _strides(v_new), None if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(),
           lse.data_ptr(), workspace.data_ptr(), size, hq, t, scale)

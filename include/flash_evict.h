@@ -281,7 +281,7 @@ typedef struct fe_cache {
  *   out: contiguous [batch, q_heads, drafts, channels], dtype of the cache;
  *   lse: FP32 [batch, q_heads, drafts], the natural logarithm of the sum of
  *   exp(scale * q.k) (-inf, with out 0, for a row that sees nothing).
- * q needs channel stride 1; k_new and v_new follow the layout rules above.
+ * q, k_new and v_new follow the layout rules above.
  * workspace: fe_tree_workspace_bytes() bytes on the cache's device, 256-byte
  * aligned, contents irrelevant.  Two launches; bitwise reproducible. */
 FE_API int64_t fe_tree_workspace_bytes(const fe_cache* cache, int64_t q_heads, int64_t drafts);
