@@ -441,14 +441,18 @@ int fe_evict_tokens(const fe_cache* cache, const fe_cache* out, int64_t budget, 
   p.recent = (int)std::min<int64_t>(recent, 0x7fffffff);
   p.row_bytes = (int)cache->channels * 2;
   p.copy = cache->mass != out->mass;
-  // CTAs per row: enough to fill the SMs with few rows, at least 1024 keys each.
+  // CTAs per row: as many as hold the row's keys, and more while they would
+  // still have 2048 keys each and the SMs are not all used.
+  auto held = [&](int ctas) {
+    return round_up((cap + ctas * fe::SHRINK_WARPS - 1) / (ctas * fe::SHRINK_WARPS), 32) * fe::SHRINK_WARPS;
+  };
   int cl = 1;
-  while (cl < 8 && rows * cl < sm_count(dev) && cap / (2 * cl) >= 1024) cl *= 2;
-  const int64_t wlen = ((cap + cl * fe::SHRINK_WARPS - 1) / (cl * fe::SHRINK_WARPS) + 31) / 32 * 32;
-  const bool smem_keys = wlen * fe::SHRINK_WARPS <= fe::SHRINK_SMEM_KEYS;
+  while (cl < fe::SHRINK_MAX_CLUSTER && held(cl) > fe::SHRINK_SMEM_KEYS) cl *= 2;
+  while (cl < fe::SHRINK_MAX_CLUSTER && rows * cl < sm_count(dev) && cap / (2 * cl) >= 2048) cl *= 2;
+  const bool smem_keys = held(cl) <= fe::SHRINK_SMEM_KEYS;
   auto kern = smem_keys ? fe::fe_shrink_kernel<true> : fe::fe_shrink_kernel<false>;
-  const int smem = smem_keys ? (int)(wlen * fe::SHRINK_WARPS * 4) : 0;
-  if ((rc = set_smem(kern, smem < 49152 ? 49152 : smem))) return rc;
+  const int smem = smem_keys ? (int)(held(cl) * 4) : 0;
+  if (smem > 32768 && (rc = set_smem(kern, fe::SHRINK_SMEM_KEYS * 4))) return rc;
   if (rows * cl > 0x7fffffff) return fail(FE_STATUS_UNSUPPORTED, "too many rows");
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));

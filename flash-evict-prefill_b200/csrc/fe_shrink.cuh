@@ -12,11 +12,18 @@
 // move nearly all of them.  A cached key carries its rotary position, so the
 // order of the slots means nothing to the attention.
 //
-// One cluster of CTAs per row, every warp a contiguous stretch of slots.  Keys
-// are order-preserving integers; the budget-th largest is found by four 8-bit
-// radix passes whose histograms are summed over distributed shared memory.
-// Holes and movers are then numbered by ballots in slot order, listed, and
-// copied by all warps of the cluster.
+// One cluster of CTAs per row, every warp a contiguous stretch of slots whose
+// order-preserving integer keys stay in shared memory (in registers the walks
+// over them have to be unrolled, and fetching that code once took longer than
+// running it: 46 us instead of XX for eight rows of 128K).  The budget-th largest key is
+// found by narrowing the range of the keys 256-fold a pass (bins of a power of
+// two from the row's smallest key, so keys that share their top bits spread over
+// the bins all the same), histograms summed over distributed shared memory,
+// ending as soon as a bin's end coincides with the budget (two passes for a row
+// one token over).  Holes and movers are numbered by ballots in slot order,
+// listed, and copied by all warps of the cluster, eight rows a warp in flight.
+// Few rows are bound by the chain of cluster barriers, large batches by the
+// moved bytes.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -46,36 +53,54 @@ struct ShrinkParams {
   int copy;  // the outputs are other buffers than the inputs
 };
 
-constexpr int SHRINK_THREADS = 512;
+constexpr int SHRINK_THREADS = 1024;
 constexpr int SHRINK_WARPS = SHRINK_THREADS / 32;
-constexpr int SHRINK_SMEM_KEYS = 49152;  // keys a CTA keeps in shared memory
+constexpr int SHRINK_MAX_CLUSTER = 8;
+// Keys a CTA holds.  (Clusters of 16 fit fewer than one to a GPC and ran eight
+// rows of 128K one after another.)
+constexpr int SHRINK_SMEM_KEYS = 49152;
+constexpr int SHRINK_LIST = 1024;  // moves listed in shared memory (one CTA a row)
 
-// Copies row `src` to row `dst` of the cache's K and V by one warp.
-__device__ __forceinline__ void shrink_move(uint8_t* kb, int64_t k_st, uint8_t* vb, int64_t v_st, int row_bytes, int src,
-                                            int dst, int lane) {
-  const uint8_t* ks = kb + src * k_st;
-  const uint8_t* vs = vb + src * v_st;
-  uint8_t* kd = kb + dst * k_st;
-  uint8_t* vd = vb + dst * v_st;
-  const int vec = row_bytes / 16;  // rows start on 16 bytes
+// Copies rows src[u] to rows dst[u], u < count <= U, of a cache's K and V by one
+// warp: all loads before the first store.
+template <int U>
+__device__ __forceinline__ void shrink_move(const ShrinkParams& p, uint8_t* kb, uint8_t* vb, const int* src,
+                                            const int* dst, int count, int lane) {
+  const int vec = p.row_bytes / 16;  // rows start on 16 bytes
   for (int c = lane; c < 2 * vec; c += 32) {
     const bool is_v = c >= vec;
-    const int o = (is_v ? c - vec : c) * 16;
-    *reinterpret_cast<uint4*>((is_v ? vd : kd) + o) = *reinterpret_cast<const uint4*>((is_v ? vs : ks) + o);
+    uint8_t* at = (is_v ? vb : kb) + (is_v ? c - vec : c) * 16;
+    const int64_t st = is_v ? p.v_st : p.k_st;
+    uint4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < count) x[u] = *reinterpret_cast<const uint4*>(at + src[u] * st);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < count) *reinterpret_cast<uint4*>(at + dst[u] * st) = x[u];
   }
-  for (int o = vec * 16 + lane * 2; o < row_bytes; o += 64) {
-    *reinterpret_cast<uint16_t*>(kd + o) = *reinterpret_cast<const uint16_t*>(ks + o);
-    *reinterpret_cast<uint16_t*>(vd + o) = *reinterpret_cast<const uint16_t*>(vs + o);
-  }
+  for (int o = vec * 16 + lane * 2; o < p.row_bytes; o += 64)
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < count) {
+        *reinterpret_cast<uint16_t*>(kb + dst[u] * p.k_st + o) = *reinterpret_cast<const uint16_t*>(kb + src[u] * p.k_st + o);
+        *reinterpret_cast<uint16_t*>(vb + dst[u] * p.v_st + o) = *reinterpret_cast<const uint16_t*>(vb + src[u] * p.v_st + o);
+      }
 }
 
-template <bool SMEM_KEYS>
-__global__ void __launch_bounds__(SHRINK_THREADS) fe_shrink_kernel(const __grid_constant__ ShrinkParams p) {
+// HELD: the keys of a CTA's slots fit its shared memory; otherwise (longer rows)
+// they are made again from the weights on every walk.
+template <bool HELD>
+__global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __grid_constant__ ShrinkParams p) {
   extern __shared__ uint32_t skeys[];
-  __shared__ uint32_t hist[2][256];
-  __shared__ int warp_count[3][SHRINK_WARPS];  // ties, holes, movers of each warp
-  __shared__ int found[2];
-  __shared__ int smax[SHRINK_WARPS], cta_max;
+  __shared__ uint32_t hist[2][257];  // the last bin counts the reserved tokens
+  __shared__ __align__(16) uint32_t sums[3][260];  // rank 0: the cluster's histogram of a pass
+  __shared__ int2 warp_count[2][SHRINK_WARPS];  // ties; holes and movers of each warp
+  __shared__ int2 cta_count[2];
+  __shared__ int found[3];
+  __shared__ int s_new[SHRINK_WARPS], cta_new;
+  __shared__ uint32_t s_lo[SHRINK_WARPS], s_hi[SHRINK_WARPS], cta_lo, cta_hi;
+  __shared__ int2 slist[SHRINK_LIST];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), size = static_cast<int>(cluster.num_blocks());
   const int row = static_cast<int>(blockIdx.x) / size;
@@ -84,6 +109,10 @@ __global__ void __launch_bounds__(SHRINK_THREADS) fe_shrink_kernel(const __grid_
   const int64_t base = static_cast<int64_t>(row) * p.capacity;
   const float* mass = p.mass_in + base;
   const int32_t* pos = p.pos_in + base;
+  auto sync = [&] {
+    if (size > 1) cluster.sync();
+    else __syncthreads();
+  };
 
   if (n <= p.budget) {
     if (p.copy) {
@@ -93,69 +122,147 @@ __global__ void __launch_bounds__(SHRINK_THREADS) fe_shrink_kernel(const __grid_
         if (p.norms_in != nullptr) p.norms_out[base + i] = p.norms_in[base + i];
       }
     }
-    cluster.sync();  // every CTA has read the length
+    sync();  // every CTA has read the length
     if (rank == 0 && tid == 0) p.len_out[row] = n;
     return;
   }
 
-  // This warp's slots: [w0, w1).
+  // This warp's slots: [w0, w1), lane l holding w0 + l, w0 + l + 32, ...
   const int wlen = ((n + size * SHRINK_WARPS - 1) / (size * SHRINK_WARPS) + 31) & ~31;
   const int w0 = min(n, (rank * SHRINK_WARPS + warp) * wlen), w1 = min(n, w0 + wlen);
+  const int steps = (w1 - w0 + 31) >> 5;
 
-  int first_reserved = 0;  // positions from here on are reserved (recent > 0)
-  if (p.recent > 0) {
-    int newest = -0x7fffffff - 1;
-    for (int i = w0 + lane; i < w1; i += 32) newest = max(newest, pos[i]);
-    newest = __reduce_max_sync(0xffffffffu, newest);
-    if (lane == 0) smax[warp] = newest;
-    __syncthreads();
-    if (tid == 0) {
-      int m = smax[0];
-      for (int w = 1; w < SHRINK_WARPS; ++w) m = max(m, smax[w]);
-      cta_max = m;
+  if (p.copy) {
+    // Everything below the budget; the holes are overwritten after a barrier.
+#pragma unroll 4
+    for (int i = rank * SHRINK_THREADS + tid; i < p.budget; i += size * SHRINK_THREADS) {
+      p.mass_out[base + i] = mass[i];
+      p.pos_out[base + i] = pos[i];
+      if (p.norms_in != nullptr) p.norms_out[base + i] = p.norms_in[base + i];
     }
-    cluster.sync();
-    newest = cta_max;
-    for (int r = 0; r < size; ++r) newest = max(newest, *cluster.map_shared_rank(&cta_max, r));
-    first_reserved = static_cast<int>(max(static_cast<int64_t>(newest) - p.recent + 1, static_cast<int64_t>(-0x80000000LL)));
   }
-  auto make_key = [&](int i) -> uint32_t {
-    if (p.recent > 0 && pos[i] >= first_reserved) return 0xFFFFFFFFu;
-    // NaN below the reserved tokens, above +inf
-    return min(order_key(mass[i]), 0xFFFFFFFEu);
-  };
+
   uint32_t* wkeys = skeys + warp * wlen;
-  auto key_at = [&](int i) -> uint32_t { return SMEM_KEYS ? wkeys[i - w0] : make_key(i); };
-  if (SMEM_KEYS)
-    for (int i = w0 + lane; i < w1; i += 32) wkeys[i - w0] = make_key(i);
+  int first_reserved = 0;  // positions from here on are reserved (recent > 0)
+  uint32_t lo = 0xFFFFFFFFu, hi = 0u;  // range of the row's weights
+  auto mass_key = [&](float m) -> uint32_t { return min(order_key(m), 0xFFFFFFFEu); };  // NaN above +inf, below the reserved
+  auto as_key = [&](uint32_t k, int at) -> uint32_t { return p.recent > 0 && at >= first_reserved ? 0xFFFFFFFFu : k; };
+  {
+    int newest = -0x7fffffff - 1;
+    // Loads of eight slots at a time, past the end from the last slot.
+    for (int j0 = 0; j0 < steps; j0 += 8) {
+      uint32_t k[8];
+      int at[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = min(w0 + (j0 + u) * 32 + lane, n - 1);
+        k[u] = __float_as_uint(mass[i]);
+        at[u] = p.recent > 0 ? pos[i] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        k[u] = mass_key(__uint_as_float(k[u]));
+        lo = min(lo, k[u]);
+        hi = max(hi, k[u]);
+        newest = max(newest, at[u]);
+        if (HELD && w0 + (j0 + u) * 32 + lane < w1) wkeys[(j0 + u) * 32 + lane] = k[u];
+      }
+    }
+    if (tid < 257) {
+      hist[0][tid] = hist[1][tid] = 0u;
+      sums[0][tid] = sums[1][tid] = sums[2][tid] = 0u;
+    }
+    newest = __reduce_max_sync(0xffffffffu, newest);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) {
+      s_new[warp] = newest;
+      s_lo[warp] = lo;
+      s_hi[warp] = hi;
+    }
+    __syncthreads();
+    newest = __reduce_max_sync(0xffffffffu, s_new[lane % SHRINK_WARPS]);
+    lo = __reduce_min_sync(0xffffffffu, s_lo[lane % SHRINK_WARPS]);
+    hi = __reduce_max_sync(0xffffffffu, s_hi[lane % SHRINK_WARPS]);
+    if (size > 1) {
+      if (tid == 0) {
+        cta_new = newest;
+        cta_lo = lo;
+        cta_hi = hi;
+      }
+      cluster.sync();
+      const int r = lane < size ? lane : 0;
+      newest = __reduce_max_sync(0xffffffffu, *cluster.map_shared_rank(&cta_new, r));
+      lo = __reduce_min_sync(0xffffffffu, *cluster.map_shared_rank(&cta_lo, r));
+      hi = __reduce_max_sync(0xffffffffu, *cluster.map_shared_rank(&cta_hi, r));
+    }
+    first_reserved =
+        static_cast<int>(max(static_cast<int64_t>(newest) - p.recent + 1, static_cast<int64_t>(-0x80000000LL)));
+    if (HELD && p.recent > 0) {
+      for (int j0 = 0; j0 < steps; j0 += 8) {
+        int at[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) at[u] = pos[min(w0 + (j0 + u) * 32 + lane, n - 1)];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (at[u] >= first_reserved && w0 + (j0 + u) * 32 + lane < w1) wkeys[(j0 + u) * 32 + lane] = 0xFFFFFFFFu;
+      }
+    }
+    __syncwarp();
+  }
+  // Calls f(slot, valid, key) for the warp's slots, 32 at a time in order.
+  auto walk = [&](auto f) {
+#pragma unroll 2
+    for (int j = 0; j < steps; ++j) {
+      const int i = w0 + j * 32 + lane;
+      uint32_t k = 0u;
+      if (i < w1) k = HELD ? wkeys[j * 32 + lane] : as_key(mass_key(mass[i]), p.recent > 0 ? pos[i] : 0);
+      f(i, i < w1, k);
+    }
+  };
 
   // ---- the budget-th largest key
-  uint32_t prefix = 0u;
-  int need = p.budget, ties = 0;
-  for (int i = tid; i < 512; i += SHRINK_THREADS) hist[i >> 8][i & 255] = 0u;
-  __syncthreads();
+  // Candidates are the keys in [lo, lo + 2^width); bins of 2^shift of them.
+  int width = 32 - __clz(hi - lo), need = p.budget, ties = 0;
+  uint32_t threshold = lo;
 #pragma unroll 1
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
+  for (int pass = 0; pass < 4; ++pass) {  // 32 bits, 8 a pass
+    const int shift = max(width - 8, 0);
     uint32_t* hh = hist[pass & 1];
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-      const int i = i0 + lane;
-      const uint32_t key = i < w1 ? key_at(i) : 0u;
-      const bool in = i < w1 && (pass == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
-      const uint32_t digit = in ? (key >> shift) & 255u : 256u;
-      // The keys crowd into few digits: add once per distinct digit of the warp.
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      if (in && (__ffs(same) - 1) == lane) atomicAdd(&hh[digit], static_cast<uint32_t>(__popc(same)));
+    walk([&](int, bool valid, uint32_t k) {
+      const bool reserved = k == 0xFFFFFFFFu;
+      const uint32_t d = k - threshold;
+      const bool in = valid && (reserved ? pass == 0 : width == 32 || (d >> width) == 0u);
+      const uint32_t bin = reserved ? 256u : d >> shift;
+      // The first candidate's bin once for all lanes that share it (weights of
+      // exactly zero can be most of a row), the others one by one.
+      const uint32_t any = __ballot_sync(0xffffffffu, in);
+      if (any == 0u) return;
+      const int first = __ffs(any) - 1;
+      const uint32_t first_bin = __shfl_sync(0xffffffffu, bin, first);  // by all lanes: not inside a condition
+      const uint32_t same = __ballot_sync(0xffffffffu, in && bin == first_bin);
+      if (lane == first) atomicAdd(&hh[bin], static_cast<uint32_t>(__popc(same)));
+      else if (in && !((same >> lane) & 1u)) atomicAdd(&hh[bin], 1u);
+    });
+    // The cluster's histogram gathers in rank 0 (three buffers: one is read, the
+    // next is added to, the one after is zeroed, between two cluster barriers).
+    if (size > 1) {
+      __syncthreads();
+      if (tid < 257 && hh[tid] != 0u) atomicAdd(cluster.map_shared_rank(&sums[pass % 3][tid], 0), hh[tid]);
     }
-    cluster.sync();
-    // Every CTA sums the clusters' histograms and finds the digit (warp 0).
+    sync();
+    if (tid >= 32 && tid < 32 + 257) {
+      hist[(pass + 1) & 1][tid - 32] = 0u;
+      sums[(pass + 2) % 3][tid - 32] = 0u;
+    }
     if (warp == 0) {
       uint32_t cnt[8];
       uint32_t mine = 0;
+      const uint32_t* from = size > 1 ? cluster.map_shared_rank(&sums[pass % 3][0], 0) : hh;
+      const uint32_t reserved = from[256];  // above every bin (only the first pass counts them)
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        cnt[u] = 0;
-        for (int r = 0; r < size; ++r) cnt[u] += *cluster.map_shared_rank(&hh[lane * 8 + u], r);
+        cnt[u] = from[lane * 8 + u];
         mine += cnt[u];
       }
       uint32_t above = mine;  // inclusive suffix sum over the lanes
@@ -164,107 +271,135 @@ __global__ void __launch_bounds__(SHRINK_THREADS) fe_shrink_kernel(const __grid_
         const uint32_t x = __shfl_down_sync(0xffffffffu, above, o);
         if (lane + o < 32) above += x;
       }
-      uint32_t upper = above - mine;  // keys in higher lanes' digits
+      uint32_t upper = reserved + above - mine;  // keys above this lane's bins
+      if (reserved >= static_cast<uint32_t>(need) && lane == 0) {
+        found[0] = 256;
+        found[1] = 0;
+        found[2] = static_cast<int>(reserved);
+      }
 #pragma unroll
       for (int u = 7; u >= 0; --u) {
         if (upper < static_cast<uint32_t>(need) && upper + cnt[u] >= static_cast<uint32_t>(need)) {
           found[0] = lane * 8 + u;
           found[1] = static_cast<int>(upper);
-          warp_count[0][0] = static_cast<int>(cnt[u]);
+          found[2] = static_cast<int>(cnt[u]);
         }
         upper += cnt[u];
       }
     }
-    // The other histogram is free: every CTA is past reading it.
-    if (warp > 0 && pass < 3)
-      for (int i = tid - 32; i < 256; i += SHRINK_THREADS - 32) hist[(pass + 1) & 1][i] = 0u;
     __syncthreads();
-    prefix |= static_cast<uint32_t>(found[0]) << shift;
+    const int bin = found[0];
     need -= found[1];
-    ties = warp_count[0][0];
+    ties = found[2];
+    if (bin == 256) {
+      threshold = 0xFFFFFFFFu;
+      break;
+    }
+    threshold += static_cast<uint32_t>(bin) << shift;
+    // Done when all keys of this bin stay, or it holds one key.
+    if (ties == need || shift == 0) break;
+    width = shift;
     __syncthreads();
   }
-  const uint32_t threshold = prefix;
   const int keep_ties = need;  // of `ties` keys equal to it, the first ones stay
+  const bool split_ties = ties > keep_ties;
 
-  auto prefix_of = [&](int which) -> int {
-    // Sum of warp_count[which] over the warps before this one, in the cluster.
-    int s = 0;
-    for (int i = lane; i < rank * SHRINK_WARPS + warp; i += 32)
-      s += *cluster.map_shared_rank(&warp_count[which][i % SHRINK_WARPS], i / SHRINK_WARPS);
-    return __reduce_add_sync(0xffffffffu, s);
+  // Sums of a pair of counts over the warps before this one, in the whole
+  // cluster; the cluster's totals in *total.
+  auto scan = [&](int which, int2 mine, int2* total) -> int2 {
+    if (lane == 0) warp_count[which][warp] = mine;
+    __syncthreads();
+    static_assert(SHRINK_WARPS == 32, "a lane per warp");
+    const int2 v = warp_count[which][lane];
+    int2 before = make_int2(__reduce_add_sync(0xffffffffu, lane < warp ? v.x : 0),
+                            __reduce_add_sync(0xffffffffu, lane < warp ? v.y : 0));
+    int2 all = make_int2(__reduce_add_sync(0xffffffffu, v.x), __reduce_add_sync(0xffffffffu, v.y));
+    if (size > 1) {
+      if (tid == 0) cta_count[which] = all;
+      cluster.sync();
+      int2 c = make_int2(0, 0);
+      if (lane < size) c = *cluster.map_shared_rank(&cta_count[which], lane);
+      before.x += __reduce_add_sync(0xffffffffu, lane < rank ? c.x : 0);
+      before.y += __reduce_add_sync(0xffffffffu, lane < rank ? c.y : 0);
+      all = make_int2(__reduce_add_sync(0xffffffffu, c.x), __reduce_add_sync(0xffffffffu, c.y));
+    }
+    *total = all;
+    return before;
   };
+  const uint32_t below = (1u << lane) - 1u;
   int tie_base = 0;
-  if (ties > keep_ties) {
+  int2 total;
+  if (split_ties) {
     int c = 0;
-    for (int i = w0 + lane; i < w1; i += 32) c += key_at(i) == threshold ? 1 : 0;
+    walk([&](int, bool valid, uint32_t k) { c += valid && k == threshold ? 1 : 0; });
     c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) warp_count[0][warp] = c;
-    cluster.sync();
-    tie_base = prefix_of(0);
+    tie_base = scan(0, make_int2(c, 0), &total).x;
   }
-  // Calls f(slot, valid, kept) for the warp's slots, 32 at a time in order.
+  // Calls f(slot, valid, kept) in order.
   auto sweep = [&](auto f) {
     int seen = tie_base;
-    for (int i0 = w0; i0 < w1; i0 += 32) {
-      const int i = i0 + lane;
-      const bool valid = i < w1;
-      const uint32_t key = valid ? key_at(i) : 0u;
-      bool keep = valid && key >= threshold;
-      if (ties > keep_ties) {
-        const bool tie = valid && key == threshold;
+    walk([&](int i, bool valid, uint32_t k) {
+      bool keep = valid && k >= threshold;
+      if (split_ties) {
+        const bool tie = valid && k == threshold;
         const uint32_t bal = __ballot_sync(0xffffffffu, tie);
-        if (tie) keep = seen + __popc(bal & ((1u << lane) - 1u)) < keep_ties;
+        if (tie) keep = seen + __popc(bal & below) < keep_ties;
         seen += __popc(bal);
       }
       f(i, valid, keep);
-    }
+    });
   };
   int nh = 0, nm = 0;
   sweep([&](int i, bool valid, bool keep) {
     nh += __popc(__ballot_sync(0xffffffffu, valid && !keep && i < p.budget));
     nm += __popc(__ballot_sync(0xffffffffu, keep && i >= p.budget));
   });
-  if (lane == 0) {
-    warp_count[1][warp] = nh;
-    warp_count[2][warp] = nm;
-  }
-  cluster.sync();
-  int hole = prefix_of(1), mover = prefix_of(2);
+  const int2 start = scan(1, make_int2(nh, nm), &total);
+  int hole = start.x, mover = start.y;
+  const int moves = total.x;  // as many holes as movers
+  // One CTA with few moves lists them in shared memory.
+  const bool local = size == 1 && moves <= SHRINK_LIST;
   int32_t* holes = p.holes + static_cast<int64_t>(row) * p.list;
   int32_t* movers = p.movers + static_cast<int64_t>(row) * p.list;
   sweep([&](int i, bool valid, bool keep) {
     const bool is_hole = valid && !keep && i < p.budget, is_mover = keep && i >= p.budget;
     const uint32_t bh = __ballot_sync(0xffffffffu, is_hole), bm = __ballot_sync(0xffffffffu, is_mover);
-    const uint32_t below = (1u << lane) - 1u;
-    if (is_hole) holes[hole + __popc(bh & below)] = i;
-    if (is_mover) movers[mover + __popc(bm & below)] = i;
+    if (is_hole) {
+      if (local) slist[hole + __popc(bh & below)].x = i;
+      else holes[hole + __popc(bh & below)] = i;
+    }
+    if (is_mover) {
+      if (local) slist[mover + __popc(bm & below)].y = i;
+      else movers[mover + __popc(bm & below)] = i;
+    }
     hole += __popc(bh);
     mover += __popc(bm);
-    if (p.copy && keep && i < p.budget) {
-      p.mass_out[base + i] = mass[i];
-      p.pos_out[base + i] = pos[i];
-      if (p.norms_in != nullptr) p.norms_out[base + i] = p.norms_in[base + i];
-    }
   });
-  int moves = 0;
-  for (int i = lane; i < size * SHRINK_WARPS; i += 32)
-    moves += *cluster.map_shared_rank(&warp_count[1][i % SHRINK_WARPS], i / SHRINK_WARPS);
-  moves = __reduce_add_sync(0xffffffffu, moves);
-  __threadfence();
-  cluster.sync();  // the lists are complete, and nobody reads a neighbour's shared memory any more
+  if (!local) __threadfence();
+  sync();  // the lists are complete, and nobody reads a neighbour's shared memory any more
   if (rank == 0 && tid == 0) p.len_out[row] = p.budget;
   const int b = row / p.Hkv, h = row - b * p.Hkv;
   uint8_t* kb = p.k + b * p.k_sb + h * p.k_sh;
   uint8_t* vb = p.v + b * p.v_sb + h * p.v_sh;
-  for (int i = rank * SHRINK_WARPS + warp; i < moves; i += size * SHRINK_WARPS) {
-    const int dst = __ldcg(holes + i), src = __ldcg(movers + i);
-    shrink_move(kb, p.k_st, vb, p.v_st, p.row_bytes, src, dst, lane);
-    if (lane == 0) {
-      p.mass_out[base + dst] = mass[src];
-      p.pos_out[base + dst] = pos[src];
-      if (p.norms_in != nullptr) p.norms_out[base + dst] = p.norms_in[base + src];
+  // Eight consecutive moves a warp: lane u < 8 knows the u-th.
+  constexpr int U = 8;
+  for (int i0 = (rank * SHRINK_WARPS + warp) * U; i0 < moves; i0 += size * SHRINK_WARPS * U) {
+    const int count = min(U, moves - i0);
+    int my_dst = 0, my_src = 0;
+    if (lane < count) {
+      my_dst = local ? slist[i0 + lane].x : __ldcg(holes + i0 + lane);
+      my_src = local ? slist[i0 + lane].y : __ldcg(movers + i0 + lane);
+      p.mass_out[base + my_dst] = mass[my_src];
+      p.pos_out[base + my_dst] = pos[my_src];
+      if (p.norms_in != nullptr) p.norms_out[base + my_dst] = p.norms_in[base + my_src];
     }
+    int src[U], dst[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      src[u] = __shfl_sync(0xffffffffu, my_src, u);
+      dst[u] = __shfl_sync(0xffffffffu, my_dst, u);
+    }
+    shrink_move<U>(p, kb, vb, src, dst, count, lane);
   }
 }
 

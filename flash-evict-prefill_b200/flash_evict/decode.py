@@ -15,6 +15,7 @@ on the device, so a step can be captured in a CUDA graph):
       rows over their budget lose the tokens of least weight, in place
 """
 import ctypes
+import functools
 import math
 
 import torch
@@ -44,7 +45,7 @@ class KVCache:
     copied, and cannot be replaced: update them in place.
     """
 
-    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "_c", "_ref", "_device_index")
+    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "device", "dtype", "_c", "_ref", "_device_index")
 
     def __init__(self, k, v, lengths, mass=None, positions=None, norms=None):
         if k.ndim != 4 or k.shape != v.shape or k.numel() == 0 or k.shape[-1] > 256:
@@ -68,6 +69,8 @@ class KVCache:
         init(self, "_c", _lib.Cache(k.data_ptr(), v.data_ptr(), k.stride(), v.stride(), ptr(mass), ptr(norms), ptr(positions),
                                     lengths.data_ptr(), b, h, c, d, _DTYPES[k.dtype]))
         init(self, "_ref", ctypes.byref(self._c))
+        init(self, "device", k.device)
+        init(self, "dtype", k.dtype)
         init(self, "_device_index", k.device.index)
 
     def __setattr__(self, name, value):
@@ -109,8 +112,18 @@ class KVCache:
         return self
 
 
-def _strides(t):
-    return (ctypes.c_int64 * 4)(*t.stride())
+@functools.lru_cache(maxsize=1024)
+def _stride_array(strides):
+    return (ctypes.c_int64 * 4)(*strides)
+
+
+def _readable(t):
+    """(tensor, its stride array): t if the kernels can read it in place, else a copy that they can."""
+    st = t.stride()
+    if st[3] != 1 or (st[0] | st[1] | st[2]) & 7 or t.data_ptr() & 15 or 0 in st:
+        t = _tma_view(t)
+        st = t.stride()
+    return t, _stride_array(st)
 
 
 def _call(fn, device_index, *args):
@@ -126,23 +139,24 @@ def _call(fn, device_index, *args):
 
 def _check_drafts(q, k_new, v_new, cache, tree, scale):
     """Checks shared by the operators that take drafted tokens; returns (tree, its batch stride, scale)."""
-    ck = cache.k
-    b, hk, _, d = ck.shape
-    if q.ndim != 4 or q.shape[0] != b or q.shape[3] != d or q.shape[1] % hk or not q.shape[1]:
+    b, hk, _, d = cache.k.shape
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != b or shape[3] != d or shape[1] % hk or not shape[1]:
         raise ValueError("q must have shape [batch, q_heads, drafts, channels], q_heads a multiple of the cache's kv_heads")
-    t = q.shape[2]
+    t = shape[2]
     if not 1 <= t <= MAX_DRAFTS:
         raise ValueError(f"between 1 and {MAX_DRAFTS} drafted tokens per call")
     shape = (b, hk, t, d)
     if k_new.shape != shape or v_new.shape != shape:
         raise ValueError("k_new and v_new must have shape [batch, kv_heads, drafts, channels]")
-    if not (q.dtype == k_new.dtype == v_new.dtype == ck.dtype) or not (q.device == k_new.device == v_new.device == ck.device):
+    device = cache.device
+    if not (q.dtype == k_new.dtype == v_new.dtype == cache.dtype) or not (q.device == k_new.device == v_new.device == device):
         raise ValueError("q, k_new, v_new and the cache must have the same device and dtype")
-    if torch.is_grad_enabled() and (q.requires_grad or k_new.requires_grad or v_new.requires_grad):
+    if (q.requires_grad or k_new.requires_grad or v_new.requires_grad) and torch.is_grad_enabled():
         raise ValueError("Inference only: no backward implementation")
     stride = 0
     if tree is not None:
-        if tree.dtype != torch.bool or tree.device != ck.device or tree.shape not in ((t, t), (b, t, t)):
+        if tree.dtype != torch.bool or tree.device != device or tree.shape not in ((t, t), (b, t, t)):
             raise ValueError("tree must be a bool tensor of shape [drafts, drafts] or [batch, drafts, drafts] on the cache's device")
         if not tree.is_contiguous():
             tree = tree.contiguous()
@@ -171,14 +185,15 @@ def tree_attention(q, k_new, v_new, cache, *, tree=None, scale=None):
     size = lib.fe_tree_workspace_bytes(cache._ref, hq, t)
     if size < 0:
         _lib.check(_lib.STATUS_UNSUPPORTED)
-    device = q.device
-    out = torch.empty((b, hq, t, d), dtype=q.dtype, device=device)
-    lse = torch.empty((b, hq, t), dtype=torch.float32, device=device)
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    q, k_new, v_new = _tma_view(q), _tma_view(k_new), _tma_view(v_new)
-    _call(lib.fe_tree_attention, cache._device_index, cache._ref, q.data_ptr(), _strides(q), k_new.data_ptr(), _strides(k_new),
-          v_new.data_ptr(), _strides(v_new), None if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(),
-          lse.data_ptr(), workspace.data_ptr(), size, hq, t, scale)
+    out = q.new_empty((b, hq, t, d))
+    lse = torch.empty((b, hq, t), dtype=torch.float32, device=q.device)
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    q, qs = _readable(q)
+    k_new, ks = _readable(k_new)
+    v_new, vs = _readable(v_new)
+    _call(lib.fe_tree_attention, cache._device_index, cache._ref, q.data_ptr(), qs, k_new.data_ptr(), ks, v_new.data_ptr(), vs,
+          None if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(), size, hq,
+          t, scale)
     return out, lse
 
 
@@ -187,9 +202,9 @@ def _check_out(cache, out):
         raise ValueError("the cache has no mass and positions")
     if out is None or out is cache:
         return cache
-    shares = [a is not None and a.data_ptr() == b.data_ptr() for a, b in ((cache.mass, out.mass), (cache.positions, out.positions),
-                                                                          (cache.lengths, out.lengths)) if b is not None]
-    if out.mass is None or (out.norms is None) != (cache.norms is None) or any(shares):
+    if out.mass is None or (out.norms is None) != (cache.norms is None) or out.mass.data_ptr() == cache.mass.data_ptr() \
+            or out.positions.data_ptr() == cache.positions.data_ptr() or out.lengths.data_ptr() == cache.lengths.data_ptr() \
+            or (out.norms is not None and out.norms.data_ptr() == cache.norms.data_ptr()):
         raise ValueError("out needs bookkeeping tensors of its own, the same ones that the cache has")
     if cache.k.data_ptr() != out.k.data_ptr() or cache.v.data_ptr() != out.v.data_ptr() or cache.k.shape != out.k.shape \
             or cache.k.dtype != out.k.dtype or cache.k.stride() != out.k.stride() or cache.v.stride() != out.v.stride():
@@ -220,7 +235,7 @@ def commit_tokens(cache, q, k_new, v_new, lse, accepted, positions, *, tree=None
     out = _check_out(cache, out)
     tree, tree_stride, scale = _check_drafts(q, k_new, v_new, cache, tree, scale)
     b, hq, t, _ = q.shape
-    device = cache.k.device
+    device = cache.device
     if lse.shape != (b, hq, t) or lse.dtype != torch.float32 or lse.device != device:
         raise ValueError("lse must be FP32 [batch, q_heads, drafts] on the cache's device")
     if accepted.ndim != 2 or accepted.shape[0] != b or not 1 <= accepted.shape[1] <= MAX_DRAFTS or accepted.dtype != torch.int32 \
@@ -234,12 +249,13 @@ def commit_tokens(cache, q, k_new, v_new, lse, accepted, positions, *, tree=None
     lib = _lib.load()
     size = lib.fe_commit_workspace_bytes(cache._ref, t)
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    k_new, v_new = _tma_view(k_new), _tma_view(v_new)
-    lse, accepted, positions = lse.contiguous(), accepted.contiguous(), positions.contiguous()
-    _call(lib.fe_commit_tokens, cache._device_index, cache._ref, out._ref, q.data_ptr(), _strides(q), k_new.data_ptr(),
-          _strides(k_new), v_new.data_ptr(), _strides(v_new), None if tree is None else tree.data_ptr(), tree_stride,
+    q, qs = _readable(q)
+    k_new, ks = _readable(k_new)
+    v_new, vs = _readable(v_new)
+    if not (lse.is_contiguous() and accepted.is_contiguous() and positions.is_contiguous()):
+        lse, accepted, positions = lse.contiguous(), accepted.contiguous(), positions.contiguous()
+    _call(lib.fe_commit_tokens, cache._device_index, cache._ref, out._ref, q.data_ptr(), qs, k_new.data_ptr(), ks,
+          v_new.data_ptr(), vs, None if tree is None else tree.data_ptr(), tree_stride,
           lse.data_ptr(), accepted.data_ptr(), accepted.shape[1], positions.data_ptr(), workspace.data_ptr(), size, hq, t,
           scale, recency_decay)
     return out
@@ -262,6 +278,6 @@ def evict_tokens(cache, budget, *, recent=0, out=None):
         raise ValueError("recent must be an integer in [0, budget]")
     lib = _lib.load()
     size = lib.fe_evict_workspace_bytes(cache._ref, budget)
-    workspace = torch.empty(size, dtype=torch.uint8, device=cache.k.device)
+    workspace = torch.empty(size, dtype=torch.uint8, device=cache.device)
     _call(lib.fe_evict_tokens, cache._device_index, cache._ref, out._ref, budget, recent, workspace.data_ptr(), size)
     return out
