@@ -132,16 +132,6 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   const int w0 = min(n, (rank * SHRINK_WARPS + warp) * wlen), w1 = min(n, w0 + wlen);
   const int steps = (w1 - w0 + 31) >> 5;
 
-  if (p.copy) {
-    // Everything below the budget; the holes are overwritten after a barrier.
-#pragma unroll 4
-    for (int i = rank * SHRINK_THREADS + tid; i < p.budget; i += size * SHRINK_THREADS) {
-      p.mass_out[base + i] = mass[i];
-      p.pos_out[base + i] = pos[i];
-      if (p.norms_in != nullptr) p.norms_out[base + i] = p.norms_in[base + i];
-    }
-  }
-
   uint32_t* wkeys = skeys + warp * wlen;
   int first_reserved = 0;  // positions from here on are reserved (recent > 0)
   uint32_t lo = 0xFFFFFFFFu, hi = 0u;  // range of the row's weights
@@ -151,21 +141,29 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
     int newest = -0x7fffffff - 1;
     // Loads of eight slots at a time, past the end from the last slot.
     for (int j0 = 0; j0 < steps; j0 += 8) {
-      uint32_t k[8];
+      float m[8], z[8];
       int at[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int i = min(w0 + (j0 + u) * 32 + lane, n - 1);
-        k[u] = __float_as_uint(mass[i]);
-        at[u] = p.recent > 0 ? pos[i] : 0;
+        m[u] = mass[i];
+        at[u] = p.recent > 0 || p.copy ? pos[i] : 0;
+        if (p.copy && p.norms_in != nullptr) z[u] = p.norms_in[base + i];
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        k[u] = mass_key(__uint_as_float(k[u]));
-        lo = min(lo, k[u]);
-        hi = max(hi, k[u]);
+        const int i = w0 + (j0 + u) * 32 + lane;
+        const uint32_t k = mass_key(m[u]);
+        lo = min(lo, k);
+        hi = max(hi, k);
         newest = max(newest, at[u]);
-        if (HELD && w0 + (j0 + u) * 32 + lane < w1) wkeys[(j0 + u) * 32 + lane] = k[u];
+        if (HELD && i < w1) wkeys[(j0 + u) * 32 + lane] = k;
+        if (p.copy && i < min(w1, p.budget)) {
+          // The evicted ones are overwritten after a barrier.
+          p.mass_out[base + i] = m[u];
+          p.pos_out[base + i] = at[u];
+          if (p.norms_in != nullptr) p.norms_out[base + i] = z[u];
+        }
       }
     }
     if (tid < 257) {
