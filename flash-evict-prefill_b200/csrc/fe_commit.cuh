@@ -50,7 +50,8 @@ struct CommitParams {
   int B, Hq, Hkv, G, T, A, D, capacity, nctas;
   int row0;            // first query row (i*G + g) of this launch
   int copy;            // mass_out, norms_out, pos_out are other buffers: fill them
-  float sc, decay_log2;
+  float sc;            // scale * log2(e)
+  double decay_log2;
   int q_vec;
   uint64_t timeout_ns;
 };
@@ -93,6 +94,61 @@ __device__ __forceinline__ int accepted_drafts(const int32_t* accepted, int A, i
     n += __popc(bal);
   }
   return n;
+}
+
+// Sum over `cols` (a multiple of 16, at most 128) query columns of one key's
+// S^T row of exp2(x * sc + bias); `release` is called once the row has been
+// read.  FULL: 128 columns, unrolled.  DRAFT: only columns whose query sees this
+// thread's draft (bit `bit` of word masks[col_query * 4]).
+template <bool FULL, bool DRAFT, typename Release>
+__device__ __forceinline__ float commit_reduce(uint32_t tS, int cols, float sc, const float* bias, const uint32_t* masks,
+                                               const uint8_t* col_query, int bit, Release release) {
+  const uint64_t sc2 = f2_pack(sc, sc);
+  uint64_t acc2[4] = {0ull, 0ull, 0ull, 0ull};
+  auto chunk = [&](int c0, const float (&x)[16]) {
+#pragma unroll
+    for (int c4 = 0; c4 < 16; c4 += 4) {
+      const float4 nb = *reinterpret_cast<const float4*>(bias + c0 + c4);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int c = c4 + 2 * u;
+        const uint64_t a2 = f2_fma(f2_pack(x[c], x[c + 1]), sc2, u == 0 ? f2_pack(nb.x, nb.y) : f2_pack(nb.z, nb.w));
+        float a0, a1;
+        f2_unpack(a2, a0, a1);
+        if (DRAFT) {
+          a0 = ((masks[col_query[c0 + c] * 4] >> bit) & 1u) ? a0 : -INFINITY;
+          a1 = ((masks[col_query[c0 + c + 1] * 4] >> bit) & 1u) ? a1 : -INFINITY;
+        }
+        acc2[(c >> 1) & 3] = f2_add(acc2[(c >> 1) & 3], f2_pack(ex2_approx(a0), ex2_approx(a1)));
+      }
+    }
+  };
+  // The next 16 columns are in flight while these are summed.
+  float xa[16], xb[16];
+  tmem_ld16_nowait(tS, reinterpret_cast<uint32_t*>(xa));
+  tmem_wait_ld16(reinterpret_cast<uint32_t*>(xa));
+  auto pair = [&](int c0, bool more_b, bool more_a) {
+    if (more_b) tmem_ld16_nowait(tS + c0 + 16, reinterpret_cast<uint32_t*>(xb));
+    else release();
+    chunk(c0, xa);
+    if (!more_b) return;
+    tmem_wait_ld16(reinterpret_cast<uint32_t*>(xb));
+    if (more_a) tmem_ld16_nowait(tS + c0 + 32, reinterpret_cast<uint32_t*>(xa));
+    else release();
+    chunk(c0 + 16, xb);
+    if (more_a) tmem_wait_ld16(reinterpret_cast<uint32_t*>(xa));
+  };
+  if (FULL) {
+#pragma unroll
+    for (int c0 = 0; c0 < 128; c0 += 32) pair(c0, true, c0 < 96);
+  } else {
+#pragma unroll 1
+    for (int c0 = 0; c0 < cols; c0 += 32) pair(c0, c0 + 16 < cols, c0 + 32 < cols);
+  }
+  float s[8];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) f2_unpack(acc2[u], s[2 * u], s[2 * u + 1]);
+  return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
 template <bool BF16, int DP>
@@ -241,7 +297,6 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
     const int wg = warp >> 2;
     const int kr = ((warp & 3) << 5) + static_cast<int>(lane);
     const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) << 5) << 16) + wg * 128;
-    const uint64_t sc2 = f2_pack(p.sc, p.sc);
     const int tid = threadIdx.x;
     constexpr int RT = C::WGS * 128;
     uint32_t li = 0;
@@ -283,12 +338,17 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         }
         for (int r = tid; r < padded; r += RT) {
           float bias = -INFINITY;  // padding, and rows that saw nothing, add 0
+          int query = 0;
           if (r < rows) {
             const int qi = (p.row0 + r) / p.G, g = p.row0 + r - qi * p.G;
             const float lse = __ldg(p.lse + (static_cast<int64_t>(b) * p.Hq + h * p.G + g) * p.T + slist[qi]);
-            if (lse != -INFINITY) bias = -fmaf(p.decay_log2, static_cast<float>(n - 1 - qi), lse * 1.4426950408889634f);
-            scol[r] = static_cast<uint8_t>(qi - i_first);
+            // Formed in 64 bits and rounded once: the rounding of its two terms
+            // would be up to 1e-6 of a weight each.
+            if (lse != -INFINITY)
+              bias = static_cast<float>(-(p.decay_log2 * (n - 1 - qi) + static_cast<double>(lse) * 1.4426950408889634));
+            query = qi - i_first;
           }
+          scol[r] = static_cast<uint8_t>(query);
           sbias[r] = bias;
         }
         if (sg.j1 == sg.tiles) {
@@ -312,7 +372,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         if (lane == 0) mbar_arrive(q_full);
         named_bar_sync(1, RT);
       }
-      const float fade = p.row0 == 0 ? exp2f(-p.decay_log2 * static_cast<float>(n)) : 1.0f;
+      const float fade = p.row0 == 0 ? static_cast<float>(exp2(-p.decay_log2 * n)) : 1.0f;
       const int nch = (rows + 127) / 128;
       for (int i = wg; i < ntile; i += C::WGS) {
         const int j = sg.j0 + i;
@@ -339,37 +399,18 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
           ++li;
           tc_fence_after();
           const int cols = (min(rows - c * 128, 128) + 15) & ~15;
-          uint64_t acc2[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) acc2[u] = 0ull;
-          for (int c0 = 0; c0 < cols; c0 += 16) {
-            float x[16];
-            tmem_ld16_nowait(tS + c0, reinterpret_cast<uint32_t*>(x));
-            tmem_wait_ld16(reinterpret_cast<uint32_t*>(x));
-            const float* bias = sbias + c * 128 + c0;
-#pragma unroll
-            for (int u = 0; u < 16; u += 2) {
-              const uint64_t a2 = f2_fma(f2_pack(x[u], x[u + 1]), sc2, f2_pack(bias[u], bias[u + 1]));
-              float a0, a1;
-              f2_unpack(a2, a0, a1);
-              if (drafts) {
-                // this thread's draft is seen by the column's query
-                const int r = c * 128 + c0 + u;
-                const uint32_t w0 = r < rows ? smask[scol[r] * 4 + (kr >> 5)] : 0u;
-                const uint32_t w1 = r + 1 < rows ? smask[scol[r + 1] * 4 + (kr >> 5)] : 0u;
-                if (!((w0 >> (kr & 31)) & 1u)) a0 = -INFINITY;
-                if (!((w1 >> (kr & 31)) & 1u)) a1 = -INFINITY;
-              }
-              acc2[(u >> 1) & 3] = f2_add(acc2[(u >> 1) & 3], f2_pack(ex2_approx(a0), ex2_approx(a1)));
-            }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[wg]);
-          float s[8];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) f2_unpack(acc2[u], s[2 * u], s[2 * u + 1]);
-          total += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+          auto release = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[wg]);
+          };
+          const float* bias = sbias + c * 128;
+          if (drafts)
+            total += commit_reduce<false, true>(tS, cols, p.sc, bias, smask + (kr >> 5), scol + c * 128, kr & 31, release);
+          else if (cols == 128)
+            total += commit_reduce<true, false>(tS, cols, p.sc, bias, nullptr, nullptr, 0, release);
+          else
+            total += commit_reduce<false, false>(tS, cols, p.sc, bias, nullptr, nullptr, 0, release);
         }
         // Aborted (watchdog): the sum is incomplete; store NaN.
         if (!ok) total = __int_as_float(0x7fffffff);

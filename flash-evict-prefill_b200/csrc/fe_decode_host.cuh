@@ -344,7 +344,7 @@ int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, 
   p.row0 = 0;
   p.copy = cache->mass != out->mass;
   p.sc = (float)((double)scale * 1.4426950408889634);
-  p.decay_log2 = (float)((double)recency_decay * 1.4426950408889634);
+  p.decay_log2 = (double)recency_decay * 1.4426950408889634;
   p.q_vec = rows_are_vectors(q, q_strides, B, q_heads, drafts, D) ? 1 : 0;
   p.timeout_ns = (uint64_t)g_watchdog_ns;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
