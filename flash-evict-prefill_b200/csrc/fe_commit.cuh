@@ -30,6 +30,7 @@
 namespace fe {
 
 constexpr int COMMIT_MAX_ACCEPTED = 128;
+constexpr int COMMIT_EXTRA = 2;  // key tiles that beginning a row costs
 
 struct CommitParams {
   const uint16_t* q;
@@ -170,12 +171,17 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
   uint64_t* drain = s_free + C::WGS;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  float* sfade = reinterpret_cast<float*>(tmem_holder + 2);
   int* scratch = reinterpret_cast<int*>(tmem_holder + 4);
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
 
   pdl_launch_dependents();
+  if (threadIdx.x == C::PRODUCER * 32) {
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tkn);
+  }
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     mbar_init(q_full, C::WGS * 4);
@@ -196,7 +202,8 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, 1, blockIdx.x, p.nctas, scratch, nullptr);
+  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, 1, COMMIT_EXTRA, blockIdx.x, p.nctas,
+                                               scratch, nullptr);
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const uint64_t TO = p.timeout_ns;
@@ -207,10 +214,6 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
 
   if (warp == C::PRODUCER) {
     // ------------------------------------------------------------ producer --
-    if (lane == 0) {
-      tma_prefetch_desc(&tk);
-      tma_prefetch_desc(&tkn);
-    }
     uint32_t it = 0;
     bool ok = true;
     while (ok && walk.next(sg)) {
@@ -303,24 +306,28 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
     bool ok = true;
     while (walk.next(sg)) {
       const int b = sg.bh / p.Hkv, h = sg.bh - b * p.Hkv;
-      const int n = accepted_drafts(p.accepted, p.A, p.T, b, nullptr);
+      // Everyone is done with the previous run's queries (every product that
+      // read them has been waited for by the warpgroup it fed).
+      named_bar_sync(1, RT);
+      const int n = accepted_drafts(p.accepted, p.A, p.T, b, warp == 0 ? slist : nullptr);
       const int rows = rows_of(b, n);
       const int ntile = sg.j1 - sg.j0;
       const int i_first = p.row0 / p.G;
+      if (tid == 0) *sfade = p.row0 == 0 ? static_cast<float>(exp2(-p.decay_log2 * n)) : 1.0f;
+      named_bar_sync(1, RT);
+      const float fade = *sfade;
       if (rows > 0) {
-        // Everyone is done with the previous run's queries (every product
-        // that read them has been waited for by the warpgroup it fed).
-        named_bar_sync(1, RT);
-        if (warp == 0) accepted_drafts(p.accepted, p.A, p.T, b, slist);
-        named_bar_sync(1, RT);
+        // Three warpgroups gather the queries while the fourth makes the biases
+        // and masks: one memory latency instead of three.
+        constexpr int QT = (C::WGS - 1) * 128;
         const int padded = (rows + 15) & ~15;
         constexpr int CPR = DP / 8;
         const uint16_t* qb = p.q + b * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
-        for (int i0 = tid; i0 < padded * CPR; i0 += RT * 4) {
+        for (int i0 = tid; wg < C::WGS - 1 && i0 < padded * CPR; i0 += QT * 4) {
           uint4 v[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * RT;
+            const int i = i0 + u * QT;
             const int r = i / CPR;
             v[u] = make_uint4(0u, 0u, 0u, 0u);
             if (r < rows) {
@@ -330,13 +337,13 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
           }
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * RT;
+            const int i = i0 + u * QT;
             const int r = i / CPR;
             if (r < padded)
               *reinterpret_cast<uint4*>(smem + C::OFF_Q + (r >> 7) * C::TILE + sw128_offset(r & 127, i % CPR, 16384)) = v[u];
           }
         }
-        for (int r = tid; r < padded; r += RT) {
+        for (int r = tid - QT; wg == C::WGS - 1 && r < padded; r += 128) {
           float bias = -INFINITY;  // padding, and rows that saw nothing, add 0
           int query = 0;
           if (r < rows) {
@@ -351,10 +358,10 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
           scol[r] = static_cast<uint8_t>(query);
           sbias[r] = bias;
         }
-        if (sg.j1 == sg.tiles) {
+        if (wg == C::WGS - 1 && sg.j1 == sg.tiles) {
           // Which drafts each accepted query of this launch sees.
           const int nq = (p.row0 + rows - 1) / p.G - i_first + 1;
-          for (int i = tid; i < nq * 4; i += RT) {
+          for (int i = tid - QT; i < nq * 4; i += 128) {
             const int t = slist[i_first + (i >> 2)], w = i & 3;
             const int cnt = min(max((p.tree == nullptr ? t + 1 : p.T) - 32 * w, 0), 32);
             uint32_t bits = cnt == 32 ? 0xffffffffu : ((1u << cnt) - 1u);
@@ -372,7 +379,6 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         if (lane == 0) mbar_arrive(q_full);
         named_bar_sync(1, RT);
       }
-      const float fade = p.row0 == 0 ? static_cast<float>(exp2(-p.decay_log2 * n)) : 1.0f;
       const int nch = (rows + 127) / 128;
       for (int i = wg; i < ntile; i += C::WGS) {
         const int j = sg.j0 + i;

@@ -24,47 +24,55 @@ struct DecSegment {
   int bh, mt, j0, j1, tiles, len;
 };
 
-// Walks the segments of one CTA's run.  A row bh has MT * tiles(bh) units (MT
-// row tiles of queries, each over all of the row's key tiles); tiles(bh) is
-// the cache's tiles and one tile of drafted tokens.
+// Walks the segments of one CTA's run.  A row bh has MT * (tiles(bh) + extra)
+// units: MT row tiles of queries, each over all of the row's key tiles (the
+// cache's and one of drafted tokens) and `extra` units of no work, which stand
+// for what a run spends on beginning and ending a row.
 struct DecWalk {
   const int32_t* lengths;
-  int capacity, mts, bh, unit, left;
+  int capacity, mts, extra, bh, unit, left;
   __device__ __forceinline__ bool next(DecSegment& s) {
-    if (left <= 0) return false;
-    s.bh = bh;
-    s.len = cache_length(lengths, bh, capacity);
-    s.tiles = (s.len + DEC_TILE - 1) / DEC_TILE + 1;
-    s.mt = unit / s.tiles;
-    s.j0 = unit - s.mt * s.tiles;
-    const int n = min(left, s.tiles - s.j0);
-    s.j1 = s.j0 + n;
-    left -= n;
-    unit += n;
-    if (unit == mts * s.tiles) {
-      unit = 0;
-      ++bh;
+    while (left > 0) {
+      s.bh = bh;
+      s.len = cache_length(lengths, bh, capacity);
+      s.tiles = (s.len + DEC_TILE - 1) / DEC_TILE + 1;
+      const int span = s.tiles + extra;
+      s.mt = unit / span;
+      s.j0 = unit - s.mt * span;
+      const int n = min(left, span - s.j0);
+      s.j1 = min(s.j0 + n, s.tiles);
+      left -= n;
+      unit += n;
+      if (unit == mts * span) {
+        unit = 0;
+        ++bh;
+      }
+      if (s.j1 > s.j0) return true;
     }
-    return true;
+    return false;
   }
 };
 
 constexpr int DEC_SCRATCH_INTS = 36;
 
+// Units that stand for a row's beginning and end in a launch of `total` key
+// tiles: with few tiles a run they would only spread the work over fewer SMs.
+__device__ __forceinline__ int dec_extra(int total, int nctas, int extra) { return total >= 4 * nctas ? extra : 0; }
+
 // Where this CTA's run starts.  All THREADS threads call it; `scratch` is
-// shared memory.  With base != nullptr the first unit of every row and the
-// total are written there (nbh + 1 values).
+// shared memory.  With base != nullptr the first unit of every row, the total
+// and the extra units are written there (nbh + 2 values).
 template <int THREADS>
-__device__ __forceinline__ DecWalk dec_walk_init(const int32_t* lengths, int nbh, int capacity, int mts, int cta,
+__device__ __forceinline__ DecWalk dec_walk_init(const int32_t* lengths, int nbh, int capacity, int mts, int extra, int cta,
                                                  int nctas, int* scratch, int32_t* base) {
   constexpr int WARPS = THREADS / 32;
   static_assert(WARPS <= 32 && THREADS % 32 == 0, "one warp scans the warps' sums");
   const int per_thread = (nbh + THREADS - 1) / THREADS;
   const int first = min(nbh, static_cast<int>(threadIdx.x) * per_thread);
   const int last = min(nbh, first + per_thread);
+  auto tiles_of = [&](int i) { return (cache_length(lengths, i, capacity) + DEC_TILE - 1) / DEC_TILE + 1; };
   int mine = 0;
-  for (int i = first; i < last; ++i)
-    mine += mts * ((cache_length(lengths, i, capacity) + DEC_TILE - 1) / DEC_TILE + 1);
+  for (int i = first; i < last; ++i) mine += mts * tiles_of(i);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int incl = mine;
 #pragma unroll
@@ -81,11 +89,14 @@ __device__ __forceinline__ DecWalk dec_walk_init(const int32_t* lengths, int nbh
     before += w < warp ? v : 0;
     total += v;
   }
-  int start = before + incl - mine;
+  DecWalk walk;
+  walk.extra = dec_extra(total, nctas, extra);
+  total += nbh * mts * walk.extra;
+  int start = before + incl - mine + first * mts * walk.extra;
   const int per = (total + nctas - 1) / nctas;
   const int lo = min(total, cta * per);
   for (int i = first; i < last; ++i) {
-    const int n = mts * ((cache_length(lengths, i, capacity) + DEC_TILE - 1) / DEC_TILE + 1);
+    const int n = mts * (tiles_of(i) + walk.extra);
     if (base != nullptr) base[i] = start;
     if (start <= lo && lo < start + n) {
       scratch[33] = i;
@@ -93,16 +104,18 @@ __device__ __forceinline__ DecWalk dec_walk_init(const int32_t* lengths, int nbh
     }
     start += n;
   }
-  if (base != nullptr && threadIdx.x == 0) base[nbh] = total;
+  if (base != nullptr && threadIdx.x == 0) {
+    base[nbh] = total;
+    base[nbh + 1] = walk.extra;
+  }
   __syncthreads();
-  DecWalk w;
-  w.lengths = lengths;
-  w.capacity = capacity;
-  w.mts = mts;
-  w.left = min(per, total - lo);
-  w.bh = w.left > 0 ? scratch[33] : 0;
-  w.unit = w.left > 0 ? scratch[34] : 0;
-  return w;
+  walk.lengths = lengths;
+  walk.capacity = capacity;
+  walk.mts = mts;
+  walk.left = min(per, total - lo);
+  walk.bh = walk.left > 0 ? scratch[33] : 0;
+  walk.unit = walk.left > 0 ? scratch[34] : 0;
+  return walk;
 }
 
 // Bytes of the 16-byte chunk `chunk` (8 elements) of row r in a 128-byte-swizzled

@@ -75,7 +75,7 @@ int tree_geometry(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t draf
   if (nbh * g->MT * tiles > 0x3fffffff) return fail(FE_STATUS_UNSUPPORTED, "problem too large");
   g->ctas = std::min<int64_t>(sms, nbh * g->MT * tiles);
   g->slots = nbh * g->MT + g->ctas;
-  g->off_stats = round_up((nbh + 1) * 4, 256);
+  g->off_stats = round_up((nbh + 2) * 4, 256);
   g->off_acc = g->off_stats + round_up(g->slots * g->R * 8, 256);
   g->bytes = g->off_acc + g->slots * g->R * g->D4 * 4;
   return FE_STATUS_OK;

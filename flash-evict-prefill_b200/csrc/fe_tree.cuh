@@ -42,7 +42,7 @@ struct TreeParams {
   const int32_t* lengths;
   uint16_t* out;  // [B, Hq, T, D] contiguous
   float* lse;     // [B, Hq, T]
-  int32_t* base;  // workspace: first unit of every row, total
+  int32_t* base;  // workspace: first unit of every row, total, extra units a row
   float2* stats;  // workspace: [slots][R] {m, l}
   float4* acc;    // workspace: [slots][D4/4][R]: consecutive rows are consecutive in memory
   int B, Hq, Hkv, G, T, D, capacity;
@@ -79,6 +79,7 @@ struct TreeCfg {
 // Lowest running max: finite, so that a row which has seen no key yet rescales
 // by 2^-huge = 0 and never forms inf - inf.
 constexpr float TREE_M0 = -3.0e38f;
+constexpr int TREE_EXTRA = 2;  // key tiles that beginning and ending a row cost
 constexpr uint32_t TREE_QBUF = 8192;  // bytes between the halves of a query tile's 64-column group
 
 // One key tile of a row's softmax (S in x).  With `masked`, only columns with
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(384, 1)
   }
   tc_fence_before();
   // Ends with a block barrier, which also publishes the barriers and TMEM.
-  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, p.MT, blockIdx.x, p.nctas, scratch,
+  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, p.MT, TREE_EXTRA, blockIdx.x, p.nctas, scratch,
                                            blockIdx.x == 0 ? p.base : nullptr);
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
@@ -619,9 +620,10 @@ __global__ void __launch_bounds__(TREE_JOIN_THREADS)
   const int quad0 = live ? pair / rows * Q : 0, r = live ? pair % rows : 0;
   const int total = p.base[p.B * p.Hkv];
   const int start = p.base[bh];
-  const int tiles = (p.base[bh + 1] - start) / p.MT;
+  const int extra = p.base[p.B * p.Hkv + 1];
+  const int span = (p.base[bh + 1] - start) / p.MT, tiles = span - extra;
   const int per = (total + p.nctas - 1) / p.nctas;
-  const int u0 = start + mt * tiles;
+  const int u0 = start + mt * span;
   const int c0 = u0 / per, n = (u0 + tiles - 1) / per - c0 + 1;
   if (n == 1) return;  // one run had the whole row and wrote it
   const int64_t slot0 = static_cast<int64_t>(item) + c0;
