@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
   }
   tc_fence_before();
   DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, 1, COMMIT_EXTRA, blockIdx.x, p.nctas,
-                                               scratch, nullptr);
+                                               scratch);
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const uint64_t TO = p.timeout_ns;

@@ -59,20 +59,25 @@ constexpr int DEC_SCRATCH_INTS = 36;
 // tiles: with few tiles a run they would only spread the work over fewer SMs.
 __device__ __forceinline__ int dec_extra(int total, int nctas, int extra) { return total >= 4 * nctas ? extra : 0; }
 
-// Where this CTA's run starts.  All THREADS threads call it; `scratch` is
-// shared memory.  With base != nullptr the first unit of every row, the total
-// and the extra units are written there (nbh + 2 values).
+// The layout of the units: first unit of the rows and their total.
+struct DecLayout {
+  int total, per, extra;  // units, units a run, extra units a row tile
+};
+
+// Sums the rows' units; every thread gets the layout and the first unit of its
+// own rows [first, last).  All THREADS threads call it (one block barrier;
+// scratch is free again after the next one).
 template <int THREADS>
-__device__ __forceinline__ DecWalk dec_walk_init(const int32_t* lengths, int nbh, int capacity, int mts, int extra, int cta,
-                                                 int nctas, int* scratch, int32_t* base) {
+__device__ __forceinline__ DecLayout dec_layout(const int32_t* lengths, int nbh, int capacity, int mts, int extra, int nctas,
+                                                int* scratch, int& first, int& last, int& start) {
   constexpr int WARPS = THREADS / 32;
   static_assert(WARPS <= 32 && THREADS % 32 == 0, "one warp scans the warps' sums");
   const int per_thread = (nbh + THREADS - 1) / THREADS;
-  const int first = min(nbh, static_cast<int>(threadIdx.x) * per_thread);
-  const int last = min(nbh, first + per_thread);
-  auto tiles_of = [&](int i) { return (cache_length(lengths, i, capacity) + DEC_TILE - 1) / DEC_TILE + 1; };
+  first = min(nbh, static_cast<int>(threadIdx.x) * per_thread);
+  last = min(nbh, first + per_thread);
   int mine = 0;
-  for (int i = first; i < last; ++i) mine += mts * tiles_of(i);
+  for (int i = first; i < last; ++i)
+    mine += mts * ((cache_length(lengths, i, capacity) + DEC_TILE - 1) / DEC_TILE + 1);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int incl = mine;
 #pragma unroll
@@ -89,30 +94,37 @@ __device__ __forceinline__ DecWalk dec_walk_init(const int32_t* lengths, int nbh
     before += w < warp ? v : 0;
     total += v;
   }
-  DecWalk walk;
-  walk.extra = dec_extra(total, nctas, extra);
-  total += nbh * mts * walk.extra;
-  int start = before + incl - mine + first * mts * walk.extra;
-  const int per = (total + nctas - 1) / nctas;
-  const int lo = min(total, cta * per);
+  DecLayout d;
+  d.extra = dec_extra(total, nctas, extra);
+  d.total = total + nbh * mts * d.extra;
+  d.per = (d.total + nctas - 1) / nctas;
+  start = before + incl - mine + first * mts * d.extra;
+  return d;
+}
+
+// Where this CTA's run starts.  All THREADS threads call it; `scratch` is
+// shared memory of DEC_SCRATCH_INTS.  Ends with a block barrier.
+template <int THREADS>
+__device__ __forceinline__ DecWalk dec_walk_init(const int32_t* lengths, int nbh, int capacity, int mts, int extra, int cta,
+                                                 int nctas, int* scratch) {
+  int first, last, start;
+  const DecLayout d = dec_layout<THREADS>(lengths, nbh, capacity, mts, extra, nctas, scratch, first, last, start);
+  const int lo = min(d.total, cta * d.per);
   for (int i = first; i < last; ++i) {
-    const int n = mts * (tiles_of(i) + walk.extra);
-    if (base != nullptr) base[i] = start;
+    const int n = mts * ((cache_length(lengths, i, capacity) + DEC_TILE - 1) / DEC_TILE + 1 + d.extra);
     if (start <= lo && lo < start + n) {
       scratch[33] = i;
       scratch[34] = lo - start;
     }
     start += n;
   }
-  if (base != nullptr && threadIdx.x == 0) {
-    base[nbh] = total;
-    base[nbh + 1] = walk.extra;
-  }
   __syncthreads();
+  DecWalk walk;
   walk.lengths = lengths;
   walk.capacity = capacity;
   walk.mts = mts;
-  walk.left = min(per, total - lo);
+  walk.extra = d.extra;
+  walk.left = min(d.per, d.total - lo);
   walk.bh = walk.left > 0 ? scratch[33] : 0;
   walk.unit = walk.left > 0 ? scratch[34] : 0;
   return walk;

@@ -56,7 +56,7 @@ int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 struct TreeGeometry {
   int heads, tile_rows, rows;  // query heads and rows per tile, rows per work item
   bool dual;
-  int64_t M, MT, R, D4, ctas, slots, off_stats, off_acc, bytes;
+  int64_t M, MT, R, D4, ctas, slots, off_acc, bytes;
 };
 
 int tree_geometry(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t drafts, int64_t capacity,
@@ -75,8 +75,7 @@ int tree_geometry(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t draf
   if (nbh * g->MT * tiles > 0x3fffffff) return fail(FE_STATUS_UNSUPPORTED, "problem too large");
   g->ctas = std::min<int64_t>(sms, nbh * g->MT * tiles);
   g->slots = nbh * g->MT + g->ctas;
-  g->off_stats = round_up((nbh + 2) * 4, 256);
-  g->off_acc = g->off_stats + round_up(g->slots * g->R * 8, 256);
+  g->off_acc = round_up(g->slots * g->R * 8, 256);
   g->bytes = g->off_acc + g->slots * g->R * g->D4 * 4;
   return FE_STATUS_OK;
 }
@@ -121,14 +120,17 @@ int launch_tree(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
   kern<<<dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, stream>>>(tq, tk, tv, tkn, tvn, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
-  // Warps that share a row's partials: with about `ctas / items` runs a row, one
-  // per two partials, up to the block's eight.
+  // Warps that share a row's partials: one per two partials (about ctas / items
+  // of them), as long as the blocks are all resident at once (two an SM).
   const int64_t items = (int64_t)p.B * p.Hkv * p.MT;
+  const int64_t groups = (p.D4 / 4 + fe::TREE_JOIN_QUADS - 1) / fe::TREE_JOIN_QUADS, pairs = p.R * groups;
+  auto blocks = [&](int splits) {
+    const int64_t per_block = 32 * (fe::TREE_JOIN_WARPS / splits);
+    return (pairs + per_block - 1) / per_block;
+  };
   int splits = 1;
-  while (splits < fe::TREE_JOIN_WARPS && splits * 2 * items < p.nctas) splits *= 2;
-  const int64_t groups = (p.D4 / 4 + fe::TREE_JOIN_QUADS - 1) / fe::TREE_JOIN_QUADS;
-  const int64_t pairs = p.R * groups, per_block = 32 * (fe::TREE_JOIN_WARPS / splits);
-  return launch_dependent(fe::fe_tree_join_kernel<BF16>, dim3((unsigned)items, (unsigned)((pairs + per_block - 1) / per_block)),
+  while (splits < fe::TREE_JOIN_WARPS && splits * 2 * items < p.nctas && blocks(2 * splits) * items <= 2 * p.nctas) splits *= 2;
+  return launch_dependent(fe::fe_tree_join_kernel<BF16>, dim3((unsigned)items, (unsigned)blocks(splits)),
                           dim3(fe::TREE_JOIN_THREADS), stream, "tree join launch", p, C::QTILES * p.tile_rows, splits);
 }
 
@@ -196,8 +198,7 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.base = reinterpret_cast<int32_t*>(ws);
-  p.stats = reinterpret_cast<float2*>(ws + g.off_stats);
+  p.stats = reinterpret_cast<float2*>(ws);
   p.acc = reinterpret_cast<float4*>(ws + g.off_acc);
   p.B = (int)B;
   p.Hq = (int)q_heads;

@@ -42,7 +42,6 @@ struct TreeParams {
   const int32_t* lengths;
   uint16_t* out;  // [B, Hq, T, D] contiguous
   float* lse;     // [B, Hq, T]
-  int32_t* base;  // workspace: first unit of every row, total, extra units a row
   float2* stats;  // workspace: [slots][R] {m, l}
   float4* acc;    // workspace: [slots][D4/4][R]: consecutive rows are consecutive in memory
   int B, Hq, Hkv, G, T, D, capacity;
@@ -251,8 +250,7 @@ __global__ void __launch_bounds__(384, 1)
   }
   tc_fence_before();
   // Ends with a block barrier, which also publishes the barriers and TMEM.
-  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, p.MT, TREE_EXTRA, blockIdx.x, p.nctas, scratch,
-                                           blockIdx.x == 0 ? p.base : nullptr);
+  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, p.MT, TREE_EXTRA, blockIdx.x, p.nctas, scratch);
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const uint64_t TO = p.timeout_ns;
@@ -608,7 +606,7 @@ __global__ void __launch_bounds__(TREE_JOIN_THREADS)
   constexpr int Q = TREE_JOIN_QUADS;
   __shared__ float4 s_acc[TREE_JOIN_WARPS][Q][32];
   __shared__ float2 s_ml[TREE_JOIN_WARPS][32];
-  pdl_wait();
+  __shared__ int scratch[TREE_JOIN_WARPS], s_start;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int split = warp % splits;
   const int quads = p.D4 / 4, groups = (quads + Q - 1) / Q;
@@ -618,13 +616,19 @@ __global__ void __launch_bounds__(TREE_JOIN_THREADS)
   const int pair = (blockIdx.y * (TREE_JOIN_WARPS / splits) + warp / splits) * 32 + lane;
   const bool live = pair < rows * groups;
   const int quad0 = live ? pair / rows * Q : 0, r = live ? pair % rows : 0;
-  const int total = p.base[p.B * p.Hkv];
-  const int start = p.base[bh];
-  const int extra = p.base[p.B * p.Hkv + 1];
-  const int span = (p.base[bh + 1] - start) / p.MT, tiles = span - extra;
-  const int per = (total + p.nctas - 1) / p.nctas;
-  const int u0 = start + mt * span;
-  const int c0 = u0 / per, n = (u0 + tiles - 1) / per - c0 + 1;
+  // Which runs had the row: from the lengths alone, before the runs are done.
+  int first, last, start;
+  const DecLayout d = dec_layout<TREE_JOIN_THREADS>(p.lengths, p.B * p.Hkv, p.capacity, p.MT, TREE_EXTRA, p.nctas, scratch,
+                                                    first, last, start);
+  for (int i = first; i < last && i <= bh; ++i) {
+    if (i == bh) s_start = start;
+    start += p.MT * ((cache_length(p.lengths, i, p.capacity) + DEC_TILE - 1) / DEC_TILE + 1 + d.extra);
+  }
+  __syncthreads();
+  const int tiles = (cache_length(p.lengths, bh, p.capacity) + DEC_TILE - 1) / DEC_TILE + 1;
+  const int u0 = s_start + mt * (tiles + d.extra);
+  const int c0 = u0 / d.per, n = (u0 + tiles - 1) / d.per - c0 + 1;
+  pdl_wait();
   if (n == 1) return;  // one run had the whole row and wrote it
   const int64_t slot0 = static_cast<int64_t>(item) + c0;
   const float2* st_row = p.stats + slot0 * p.R + r;
