@@ -20,9 +20,11 @@
 // its drafts.  Four warpgroups take every fourth tile of a run, each with its
 // own 128-column S^T buffer; one warp streams K tiles by TMA, one issues the
 // products.  The queries of a run stay in shared memory; more than ROWS of
-// them take further launches.  fe_commit_append_kernel then writes the accepted
-// rows: a launch of its own because it changes the lengths that every CTA of
-// the first one reads.
+// them take further launches.  Two more warps append the accepted rows of the
+// runs that end a row, and wait only for the new tokens' weights.  (In the
+// warpgroup that sums them the appending cost the loop over the tiles its
+// registers: 33 -> 43 us for the batch of 16.)  Every CTA reads the lengths, so in place they are
+// written by the last CTA to finish (a counter in the cache, back at zero then).
 #pragma once
 
 #include "fe_decode.cuh"
@@ -46,11 +48,24 @@ struct CommitParams {
   float* mass_out;
   float* norms_out;
   int32_t* pos_out;
-  float* new_mass;     // workspace [B*Hkv, T]: summed weight of each draft
-  int32_t* old_lengths;  // workspace [B*Hkv]
+  float* new_mass;       // workspace [B*Hkv, T]: weight of each draft so far, between launches
+  int32_t* new_lengths;  // [B*Hkv]: the output lengths, or (in place) workspace
+  int32_t* len_out;      // in place: the lengths, written by the last CTA
+  int32_t* sync;         // in place: CTAs that are done, 0 between launches
+  const uint16_t* k_new;
+  int64_t kn_sb, kn_sh, kn_st;
+  const uint16_t* v_new;
+  int64_t vn_sb, vn_sh, vn_st;
+  uint16_t* k;
+  int64_t k_sb, k_sh, k_st;
+  uint16_t* v;
+  int64_t v_sb, v_sh, v_st;
+  const int32_t* new_positions;  // [B, T]
   int B, Hq, Hkv, G, T, A, D, capacity, nctas;
   int row0;            // first query row (i*G + g) of this launch
+  int last;            // the last launch: append
   int copy;            // mass_out, norms_out, pos_out are other buffers: fill them
+  int rows_vec;        // K/V rows can be moved 16 bytes at a time
   float sc;            // scale * log2(e)
   double decay_log2;
   int q_vec;
@@ -71,15 +86,18 @@ struct CommitCfg {
   static constexpr int OFF_MASK = OFF_BIAS + ROWS * 4;                       // uint32[128][4]
   static constexpr int OFF_LIST = OFF_MASK + COMMIT_MAX_ACCEPTED * 16;      // int[128]
   static constexpr int OFF_COL = OFF_LIST + COMMIT_MAX_ACCEPTED * 4;        // uint8[ROWS]
-  static constexpr int OFF_BAR = OFF_COL + ROWS;
-  // q_full, k_full[S], k_empty[S], s_full[WGS], s_free[WGS], drain
-  static constexpr int NBAR = 1 + 2 * STAGES + 2 * WGS + 1;
+  static constexpr int OFF_NEW = OFF_COL + ROWS;                            // float[2][128]: weights of new tokens
+  static constexpr int OFF_APP = OFF_NEW + 2 * 128 * 4;                     // int list[128], float norm[128]
+  static constexpr int OFF_BAR = OFF_APP + COMMIT_MAX_ACCEPTED * 8;
+  // q_full, k_full[S], k_empty[S], s_full[WGS], s_free[WGS], drain, new_full[2], new_empty[2]
+  static constexpr int NBAR = 1 + 2 * STAGES + 2 * WGS + 1 + 4;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_MISC + 16 + DEC_SCRATCH_INTS * 4 + 1024;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int PRODUCER = WGS * 4;
   static constexpr int ISSUER = WGS * 4 + 1;
-  static constexpr int THREADS = (WGS * 4 + 2) * 32;
+  static constexpr int APPEND = WGS * 4 + 2;  // two warps
+  static constexpr int THREADS = (WGS * 4 + 4) * 32;
 };
 
 // Number of accepted drafts of sequence b, by one converged warp; with list !=
@@ -152,6 +170,74 @@ __device__ __forceinline__ float commit_reduce(uint32_t tS, int cols, float sc, 
   return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
+// Appends the K/V rows of cache row bh's accepted drafts, with their norms and
+// positions, by two warps (64 threads), eight rows a warp in flight.  The norms
+// are left in shared memory for the weights that follow.
+template <bool BF16>
+__device__ __forceinline__ void commit_append_rows(const CommitParams& p, int bh, int b, int h, int len, int fit,
+                                                   const int* list, float* norms, int warp, int lane) {
+  constexpr int U = 8;
+  const int64_t base = static_cast<int64_t>(bh) * p.capacity;
+  const uint16_t* kn = p.k_new + b * p.kn_sb + h * p.kn_sh;
+  const uint16_t* vn = p.v_new + b * p.vn_sb + h * p.vn_sh;
+  uint16_t* kc = p.k + b * p.k_sb + h * p.k_sh;
+  uint16_t* vc = p.v + b * p.v_sb + h * p.v_sh;
+  for (int i0 = warp * U; i0 < fit; i0 += 2 * U) {
+    const int count = min(U, fit - i0);
+    float norm[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) norm[u] = 0.f;
+    if (p.rows_vec) {
+      const int cpr = p.D / 8;
+      for (int c = lane; c < 2 * cpr; c += 32) {
+        const bool is_v = c >= cpr;
+        const int o = (is_v ? c - cpr : c) * 8;
+        uint4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int j = list[i0 + min(u, count - 1)];
+          x[u] = *reinterpret_cast<const uint4*>((is_v ? vn + j * p.vn_st : kn + j * p.kn_st) + o);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t slot = len + i0 + u;
+          if (u < count) *reinterpret_cast<uint4*>((is_v ? vc + slot * p.v_st : kc + slot * p.k_st) + o) = x[u];
+          if (is_v) {
+            const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              norm[u] += fabsf(elem_to_float<BF16>(static_cast<uint16_t>(w[e]))) +
+                         fabsf(elem_to_float<BF16>(static_cast<uint16_t>(w[e] >> 16)));
+          }
+        }
+      }
+    } else {
+      for (int c = lane; c < p.D; c += 32)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (u >= count) continue;
+          const int64_t slot = len + i0 + u;
+          const int j = list[i0 + u];
+          kc[slot * p.k_st + c] = kn[j * p.kn_st + c];
+          const uint16_t e = vn[j * p.vn_st + c];
+          vc[slot * p.v_st + c] = e;
+          norm[u] += fabsf(elem_to_float<BF16>(e));
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) norm[u] += __shfl_xor_sync(0xffffffffu, norm[u], o);
+      if (lane == u && u < count) {
+        const int64_t at = base + len + i0 + u;
+        if (p.norms_out != nullptr) p.norms_out[at] = norm[u];
+        norms[i0 + u] = p.norms_out != nullptr ? norm[u] : 1.0f;
+        p.pos_out[at] = __ldg(p.new_positions + static_cast<int64_t>(b) * p.T + list[i0 + u]);
+      }
+    }
+  }
+}
+
 template <bool BF16, int DP>
 __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
     fe_commit_mass_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tkn,
@@ -169,6 +255,8 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
   uint64_t* s_full = k_empty + C::STAGES;
   uint64_t* s_free = s_full + C::WGS;
   uint64_t* drain = s_free + C::WGS;
+  uint64_t* new_full = drain + 1;
+  uint64_t* new_empty = new_full + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   float* sfade = reinterpret_cast<float*>(tmem_holder + 2);
@@ -177,7 +265,6 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
 
-  pdl_launch_dependents();
   if (threadIdx.x == C::PRODUCER * 32) {
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tkn);
@@ -193,6 +280,10 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
       mbar_init(&s_full[w], 1);
       mbar_init(&s_free[w], 4);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&new_full[i], 4);
+      mbar_init(&new_empty[i], 2);
+    }
     mbar_init(drain, 1);
     fence_mbar_init();
   }
@@ -207,8 +298,6 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const uint64_t TO = p.timeout_ns;
-  if (blockIdx.x == 0 && p.row0 == 0)
-    for (int i = threadIdx.x; i < p.B * p.Hkv; i += C::THREADS) p.old_lengths[i] = cache_length(p.lengths, i, p.capacity);
   DecSegment sg;
   auto rows_of = [&](int b, int n) { return min(max(n * p.G - p.row0, 0), C::ROWS); };
 
@@ -295,6 +384,41 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
       umma_commit(drain);
       mbar_wait_inflight(drain, 0, TO);
     }
+  } else if (warp >= C::APPEND) {
+    // -------------------------------------------------------------- append --
+    const int w = warp - C::APPEND;
+    int* list = reinterpret_cast<int*>(smem + C::OFF_APP);
+    float* norms = reinterpret_cast<float*>(list + COMMIT_MAX_ACCEPTED);
+    uint32_t nrow = 0;  // rows whose draft tile this run had
+    bool ok = true;
+    while (p.last && walk.next(sg)) {
+      if (sg.j1 != sg.tiles) continue;
+      const int b = sg.bh / p.Hkv, h = sg.bh - b * p.Hkv;
+      named_bar_sync(2, 64);  // both warps are done with the previous row's list
+      const int n = accepted_drafts(p.accepted, p.A, p.T, b, w == 0 ? list : nullptr);
+      named_bar_sync(2, 64);
+      const int fit = min(n, p.capacity - sg.len);
+      commit_append_rows<BF16>(p, sg.bh, b, h, sg.len, fit, list, norms, w, static_cast<int>(lane));
+      named_bar_sync(2, 64);
+      if (ok) ok = warp_all(mbar_wait(&new_full[nrow & 1], (nrow >> 1) & 1, TO, abort_flag));
+      const float* fresh = reinterpret_cast<const float*>(smem + C::OFF_NEW) + (nrow & 1) * 128;
+      for (int i = w * 32 + static_cast<int>(lane); i < fit; i += 64)
+        p.mass_out[static_cast<int64_t>(sg.bh) * p.capacity + sg.len + i] =
+            ok ? norms[i] * fresh[list[i]] : __int_as_float(0x7fffffff);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&new_empty[nrow & 1]);
+      ++nrow;
+      if (w == 0) {
+        bool bad = false;
+        if (h == 0)
+          for (int a = lane; a < p.A; a += 32) bad = bad || __ldg(p.accepted + static_cast<int64_t>(b) * p.A + a) >= p.T;
+        if (bad) raise_status(FE_STATUS_BAD_INDEX);
+        if (lane == 0) {
+          p.new_lengths[sg.bh] = sg.len + fit;
+          if (fit < n) raise_status(FE_STATUS_CACHE_FULL);
+        }
+      }
+    }
   } else {
     // ------------------------------------------------ reduce (thread = key) --
     const int wg = warp >> 2;
@@ -302,9 +426,9 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
     const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) << 5) << 16) + wg * 128;
     const int tid = threadIdx.x;
     constexpr int RT = C::WGS * 128;
-    uint32_t li = 0;
+    uint32_t li = 0, nrow = 0;  // S^T tiles of this warpgroup; rows whose draft tile the run had
     bool ok = true;
-    while (walk.next(sg)) {
+    for (; walk.next(sg); nrow += sg.j1 == sg.tiles) {
       const int b = sg.bh / p.Hkv, h = sg.bh - b * p.Hkv;
       // Everyone is done with the previous run's queries (every product that
       // read them has been waited for by the warpgroup it fed).
@@ -420,9 +544,15 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         }
         // Aborted (watchdog): the sum is incomplete; store NaN.
         if (!ok) total = __int_as_float(0x7fffffff);
-        if (live) {
-          if (drafts) p.new_mass[at_new] = mass + total;
-          else p.mass_out[at] = fmaf(norm, total, mass * fade);
+        if (live && !drafts) p.mass_out[at] = fmaf(norm, total, mass * fade);
+        if (drafts && p.last) {
+          // Hand the new tokens' weights to the appending warps.
+          if (nrow >= 2 && ok) ok = warp_all(mbar_wait(&new_empty[nrow & 1], ((nrow >> 1) - 1) & 1, TO, abort_flag));
+          reinterpret_cast<float*>(smem + C::OFF_NEW)[(nrow & 1) * 128 + kr] = mass + total;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&new_full[nrow & 1]);
+        } else if (drafts && live) {
+          p.new_mass[at_new] = mass + total;
         }
       }
     }
@@ -435,84 +565,17 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-}
-
-struct AppendParams {
-  const uint16_t* k_new;
-  int64_t kn_sb, kn_sh, kn_st;
-  const uint16_t* v_new;
-  int64_t vn_sb, vn_sh, vn_st;
-  uint16_t* k;
-  int64_t k_sb, k_sh, k_st;
-  uint16_t* v;
-  int64_t v_sb, v_sh, v_st;
-  const int32_t* accepted;       // [B, A]
-  const int32_t* new_positions;  // [B, T]
-  const float* new_mass;
-  const int32_t* old_lengths;
-  float* mass;
-  float* norms;  // or null
-  int32_t* positions;
-  int32_t* lengths;
-  int Hkv, T, A, D, capacity;
-  int vec;  // rows can be moved 16 bytes at a time
-};
-
-constexpr int APPEND_THREADS = 128;
-
-// CTA (slice, kv head, sequence); a warp moves one accepted row at a time.
-template <bool BF16>
-__global__ void __launch_bounds__(APPEND_THREADS) fe_commit_append_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ int list[COMMIT_MAX_ACCEPTED];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int bh = b * p.Hkv + h;
-  const int n = accepted_drafts(p.accepted, p.A, p.T, b, warp == 0 ? list : nullptr);
-  __syncthreads();
-  pdl_wait();
-  const int len = p.old_lengths[bh];
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    p.lengths[bh] = min(len + n, p.capacity);
-    if (len + n > p.capacity) raise_status(FE_STATUS_CACHE_FULL);
-    if (h == 0)
-      for (int a = 0; a < p.A; ++a)
-        if (p.accepted[static_cast<int64_t>(b) * p.A + a] >= p.T) raise_status(FE_STATUS_BAD_INDEX);
-  }
-  constexpr int WARPS = APPEND_THREADS / 32;
-  for (int i = blockIdx.x * WARPS + warp; i < n; i += gridDim.x * WARPS) {
-    const int slot = len + i;
-    if (slot >= p.capacity) break;
-    const int j = list[i];
-    const uint16_t* ks = p.k_new + b * p.kn_sb + h * p.kn_sh + j * p.kn_st;
-    const uint16_t* vs = p.v_new + b * p.vn_sb + h * p.vn_sh + j * p.vn_st;
-    uint16_t* kd = p.k + b * p.k_sb + h * p.k_sh + slot * p.k_st;
-    uint16_t* vd = p.v + b * p.v_sb + h * p.v_sh + slot * p.v_st;
-    float norm = 0.f;
-    if (p.vec) {
-      for (int c = lane * 8; c < p.D; c += 256) {
-        *reinterpret_cast<uint4*>(kd + c) = *reinterpret_cast<const uint4*>(ks + c);
-        const uint4 w = *reinterpret_cast<const uint4*>(vs + c);
-        *reinterpret_cast<uint4*>(vd + c) = w;
-        const uint16_t* e = reinterpret_cast<const uint16_t*>(&w);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) norm += fabsf(elem_to_float<BF16>(e[u]));
-      }
-    } else {
-      for (int c = lane; c < p.D; c += 32) {
-        kd[c] = ks[c];
-        const uint16_t e = vs[c];
-        vd[c] = e;
-        norm += fabsf(elem_to_float<BF16>(e));
-      }
+  if (p.last && !p.copy) {
+    // In place: everyone has read the lengths once every CTA has come here.
+    if (threadIdx.x == 0) {
+      __threadfence();
+      scratch[0] = atomicAdd(p.sync, 1) == static_cast<int>(gridDim.x) - 1;
+      __threadfence();
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, o);
-    if (lane == 0) {
-      const int64_t at = static_cast<int64_t>(bh) * p.capacity + slot;
-      const float m = p.new_mass[static_cast<int64_t>(bh) * p.T + j];
-      p.mass[at] = p.norms != nullptr ? norm * m : m;
-      if (p.norms != nullptr) p.norms[at] = norm;
-      p.positions[at] = p.new_positions[static_cast<int64_t>(b) * p.T + j];
+    __syncthreads();
+    if (scratch[0]) {
+      for (int i = threadIdx.x; i < p.B * p.Hkv; i += C::THREADS) p.len_out[i] = __ldcg(p.new_lengths + i);
+      if (threadIdx.x == 0) *p.sync = 0;
     }
   }
 }

@@ -262,6 +262,7 @@ int launch_commit(const CUtensorMap& tk, const CUtensorMap& tkn, fe::CommitParam
   // The accepted count is on the device; A is its most.
   for (int64_t row0 = 0; row0 == 0 || row0 < (int64_t)p.A * p.G; row0 += C::ROWS) {
     p.row0 = (int)row0;
+    p.last = row0 + C::ROWS >= (int64_t)p.A * p.G;
     kern<<<dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, stream>>>(tk, tkn, p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "commit launch");
@@ -308,7 +309,7 @@ int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, 
   if (workspace_bytes < commit_workspace(cache, drafts, &off_lengths))
     return fail(FE_STATUS_INVALID, "workspace too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 4) return fail(FE_STATUS_UNSUPPORTED, "workspace must be 4-byte aligned");
-  if (H > 65535 || B > 65535) return fail(FE_STATUS_UNSUPPORTED, "problem too large");
+  if (cache->mass == out->mass && !cache->sync) return fail(FE_STATUS_INVALID, "the cache has no sync word");
   const int64_t units = B * H * ((cache->capacity + fe::DEC_TILE - 1) / fe::DEC_TILE + 1);
   if (units > 0x3fffffff) return fail(FE_STATUS_UNSUPPORTED, "problem too large");
   int dev = 0;
@@ -332,7 +333,22 @@ int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, 
   p.norms_out = out->norms;
   p.pos_out = out->positions;
   p.new_mass = reinterpret_cast<float*>(ws);
-  p.old_lengths = reinterpret_cast<int32_t*>(ws + off_lengths);
+  p.copy = cache->mass != out->mass;
+  p.new_lengths = p.copy ? out->lengths : reinterpret_cast<int32_t*>(ws + off_lengths);
+  p.len_out = out->lengths;
+  p.sync = cache->sync;
+  p.k_new = static_cast<const uint16_t*>(k_new);
+  p.kn_sb = k_new_strides[0], p.kn_sh = k_new_strides[1], p.kn_st = k_new_strides[2];
+  p.v_new = static_cast<const uint16_t*>(v_new);
+  p.vn_sb = v_new_strides[0], p.vn_sh = v_new_strides[1], p.vn_st = v_new_strides[2];
+  p.k = static_cast<uint16_t*>(cache->k);
+  p.k_sb = cache->k_strides[0], p.k_sh = cache->k_strides[1], p.k_st = cache->k_strides[2];
+  p.v = static_cast<uint16_t*>(cache->v);
+  p.v_sb = cache->v_strides[0], p.v_sh = cache->v_strides[1], p.v_st = cache->v_strides[2];
+  p.new_positions = new_positions;
+  p.rows_vec = rows_are_vectors(k_new, k_new_strides, B, H, drafts, D) && rows_are_vectors(v_new, v_new_strides, B, H, drafts, D) &&
+               rows_are_vectors(cache->k, cache->k_strides, B, H, cache->capacity, D) &&
+               rows_are_vectors(cache->v, cache->v_strides, B, H, cache->capacity, D);
   p.B = (int)B;
   p.Hq = (int)q_heads;
   p.Hkv = (int)H;
@@ -343,7 +359,6 @@ int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, 
   p.capacity = (int)cache->capacity;
   p.nctas = (int)std::min<int64_t>(sm_count(dev), units);
   p.row0 = 0;
-  p.copy = cache->mass != out->mass;
   p.sc = (float)((double)scale * 1.4426950408889634);
   p.decay_log2 = (double)recency_decay * 1.4426950408889634;
   p.q_vec = rows_are_vectors(q, q_strides, B, q_heads, drafts, D) ? 1 : 0;
@@ -355,35 +370,7 @@ int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, 
                         : dp == 128 ? launch_commit<true, 128>(tk, tkn, p, s) : launch_commit<true, 256>(tk, tkn, p, s))
             : (dp == 64 ? launch_commit<false, 64>(tk, tkn, p, s)
                         : dp == 128 ? launch_commit<false, 128>(tk, tkn, p, s) : launch_commit<false, 256>(tk, tkn, p, s));
-  if (rc) return rc;
-  fe::AppendParams a;
-  a.k_new = static_cast<const uint16_t*>(k_new);
-  a.kn_sb = k_new_strides[0], a.kn_sh = k_new_strides[1], a.kn_st = k_new_strides[2];
-  a.v_new = static_cast<const uint16_t*>(v_new);
-  a.vn_sb = v_new_strides[0], a.vn_sh = v_new_strides[1], a.vn_st = v_new_strides[2];
-  a.k = static_cast<uint16_t*>(cache->k);
-  a.k_sb = cache->k_strides[0], a.k_sh = cache->k_strides[1], a.k_st = cache->k_strides[2];
-  a.v = static_cast<uint16_t*>(cache->v);
-  a.v_sb = cache->v_strides[0], a.v_sh = cache->v_strides[1], a.v_st = cache->v_strides[2];
-  a.accepted = accepted;
-  a.new_positions = new_positions;
-  a.new_mass = p.new_mass;
-  a.old_lengths = p.old_lengths;
-  a.mass = out->mass;
-  a.norms = out->norms;
-  a.positions = out->positions;
-  a.lengths = out->lengths;
-  a.Hkv = p.Hkv;
-  a.T = p.T;
-  a.A = p.A;
-  a.D = p.D;
-  a.capacity = p.capacity;
-  a.vec = rows_are_vectors(k_new, k_new_strides, B, H, drafts, D) && rows_are_vectors(v_new, v_new_strides, B, H, drafts, D) &&
-          rows_are_vectors(cache->k, cache->k_strides, B, H, cache->capacity, D) &&
-          rows_are_vectors(cache->v, cache->v_strides, B, H, cache->capacity, D);
-  const dim3 grid((unsigned)((max_accepted + 3) / 4), (unsigned)H, (unsigned)B);
-  return bf16 ? launch_dependent(fe::fe_commit_append_kernel<true>, grid, dim3(fe::APPEND_THREADS), s, "append launch", a)
-              : launch_dependent(fe::fe_commit_append_kernel<false>, grid, dim3(fe::APPEND_THREADS), s, "append launch", a);
+  return rc;
 }
 
 int64_t fe_evict_workspace_bytes(const fe_cache* cache, int64_t budget) {

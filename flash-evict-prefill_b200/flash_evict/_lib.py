@@ -42,7 +42,7 @@ _F32 = ctypes.c_float
 class Cache(ctypes.Structure):
     """fe_cache of include/flash_evict.h."""
     _fields_ = [("k", _VP), ("v", _VP), ("k_strides", _I64 * 4), ("v_strides", _I64 * 4), ("mass", _VP),
-                ("norms", _VP), ("positions", _VP), ("lengths", _VP), ("batch", _I64), ("kv_heads", _I64),
+                ("norms", _VP), ("positions", _VP), ("lengths", _VP), ("sync", _VP), ("batch", _I64), ("kv_heads", _I64),
                 ("capacity", _I64), ("channels", _I64), ("dtype", _INT)]
 
 

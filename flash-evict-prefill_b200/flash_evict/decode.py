@@ -45,7 +45,7 @@ class KVCache:
     copied, and cannot be replaced: update them in place.
     """
 
-    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "device", "dtype", "_c", "_ref", "_device_index")
+    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "device", "dtype", "_sync", "_c", "_ref", "_device_index")
 
     def __init__(self, k, v, lengths, mass=None, positions=None, norms=None):
         if k.ndim != 4 or k.shape != v.shape or k.numel() == 0 or k.shape[-1] > 256:
@@ -66,8 +66,9 @@ class KVCache:
             init(self, name, t)
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         b, h, c, d = k.shape
+        init(self, "_sync", None if mass is None else torch.zeros(1, dtype=torch.int32, device=k.device))
         init(self, "_c", _lib.Cache(k.data_ptr(), v.data_ptr(), k.stride(), v.stride(), ptr(mass), ptr(norms), ptr(positions),
-                                    lengths.data_ptr(), b, h, c, d, _DTYPES[k.dtype]))
+                                    lengths.data_ptr(), ptr(self._sync), b, h, c, d, _DTYPES[k.dtype]))
         init(self, "_ref", ctypes.byref(self._c))
         init(self, "device", k.device)
         init(self, "dtype", k.dtype)

@@ -269,6 +269,7 @@ typedef struct fe_cache {
   float* norms;       /* ||v||_1 of the slot, or NULL: weights are not scaled  */
   int32_t* positions; /* position of the token in its sequence                 */
   int32_t* lengths;
+  int32_t* sync;      /* one word, zero, for fe_commit_tokens in place (it is zero again after) */
   int64_t batch, kv_heads, capacity, channels;
   int dtype;
 } fe_cache;

@@ -14,7 +14,7 @@ from test_streaming_cpu import tiny_model
 
 def c_cache(**kw):
     fields = dict(k=256, v=256, k_strides=(512, 256, 8, 1), v_strides=(512, 256, 8, 1), mass=256, norms=256, positions=256,
-                  lengths=256, batch=1, kv_heads=2, capacity=32, channels=8, dtype=_lib.DTYPE_F16)
+                  lengths=256, sync=256, batch=1, kv_heads=2, capacity=32, channels=8, dtype=_lib.DTYPE_F16)
     fields.update(kw)
     c = _lib.Cache()
     for name, value in fields.items():
@@ -53,6 +53,7 @@ def test_c_abi_refusals_without_a_gpu():
     assert commit(c_cache(), c_cache(**{**other, "mass": 256})) == _lib.STATUS_INVALID and b"share all" in lib.fe_last_error()
     assert commit(c_cache(norms=None), c_cache(**other)) == _lib.STATUS_INVALID and b"norms" in lib.fe_last_error()
     assert commit(c_cache(mass=None), c_cache()) == _lib.STATUS_INVALID and b"mass" in lib.fe_last_error()
+    assert commit(c_cache(sync=None), c_cache()) == _lib.STATUS_INVALID and b"sync" in lib.fe_last_error()
     assert commit(c_cache(), c_cache(), accepted=0) == _lib.STATUS_INVALID
     assert commit(c_cache(), c_cache(), accepted=129) == _lib.STATUS_INVALID
     assert commit(c_cache(), c_cache(), decay=-1.0) == _lib.STATUS_INVALID and b"recency_decay" in lib.fe_last_error()
