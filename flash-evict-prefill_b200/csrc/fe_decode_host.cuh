@@ -33,6 +33,32 @@ int check_cache(const fe_cache* c) {
   return FE_STATUS_OK;
 }
 
+// The layout fields of a cache (everything the tensor maps depend on).
+uint64_t layout_hash(const fe_cache* c) {
+  const uint64_t f[] = {reinterpret_cast<uint64_t>(c->k), reinterpret_cast<uint64_t>(c->v), (uint64_t)c->k_strides[0],
+                        (uint64_t)c->k_strides[1], (uint64_t)c->k_strides[2], (uint64_t)c->k_strides[3],
+                        (uint64_t)c->v_strides[0], (uint64_t)c->v_strides[1], (uint64_t)c->v_strides[2],
+                        (uint64_t)c->v_strides[3], (uint64_t)c->batch, (uint64_t)c->kv_heads, (uint64_t)c->capacity,
+                        (uint64_t)c->channels, (uint64_t)c->dtype};
+  uint64_t h = 1469598103934665603ull;
+  for (uint64_t x : f) h = (h ^ x) * 1099511628211ull ^ (h >> 29);
+  return h | 1;  // 0 marks maps that were never made
+}
+
+// The cache's tensor maps: those that fe_cache_prepare left in it, as long as
+// they are of this layout, else made here.  tv may be null.
+int cache_maps(const fe_cache* c, CUtensorMap* tk, CUtensorMap* tv) {
+  static_assert(sizeof(CUtensorMap) == sizeof(c->map_k), "a tensor map is 128 bytes");
+  if (c->maps_of != 0 && c->maps_of == layout_hash(c)) {
+    memcpy(tk, c->map_k, sizeof(*tk));
+    if (tv) memcpy(tv, c->map_v, sizeof(*tv));
+    return FE_STATUS_OK;
+  }
+  int rc = make_map(tk, c->k, c->k_strides, c->batch, c->kv_heads, c->capacity, c->channels, c->dtype, "cache k");
+  if (rc || !tv) return rc;
+  return make_map(tv, c->v, c->v_strides, c->batch, c->kv_heads, c->capacity, c->channels, c->dtype, "cache v");
+}
+
 int check_drafts(const fe_cache* c, int64_t q_heads, int64_t drafts) {
   if (q_heads < 1 || q_heads % c->kv_heads) return fail(FE_STATUS_INVALID, "q_heads must be divisible by kv_heads");
   if (drafts < 1) return fail(FE_STATUS_INVALID, "at least one drafted token");
@@ -55,7 +81,7 @@ int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 // workspace query and the launch agree.
 struct TreeGeometry {
   int heads, tile_rows, rows;  // query heads and rows per tile, rows per work item
-  bool dual;
+  bool dual, cluster;
   int64_t M, MT, R, D4, ctas, slots, off_acc, bytes;
 };
 
@@ -74,9 +100,15 @@ int tree_geometry(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t draf
   const int64_t tiles = (capacity + fe::DEC_TILE - 1) / fe::DEC_TILE + 1;
   if (nbh * g->MT * tiles > 0x3fffffff) return fail(FE_STATUS_UNSUPPORTED, "problem too large");
   g->ctas = std::min<int64_t>(sms, nbh * g->MT * tiles);
+  // A cluster of eight per item instead of all SMs and a second launch: about
+  // 4 us less, for (tiles/8 - items*tiles/SMs) more tiles of 1.2 us in a row.
+  // (8 rows, one token: 4000 keys 13.2 us against 16, 6000 keys 16.1 for both.)
+  const int64_t items = nbh * g->MT;
+  g->cluster = !g->dual && items * (fe::TREE_CLUSTER + 1) <= sms &&
+               2 * tiles * (sms - items * fe::TREE_CLUSTER) <= 7 * fe::TREE_CLUSTER * sms;
   g->slots = nbh * g->MT + g->ctas;
   g->off_acc = round_up(g->slots * g->R * 8, 256);
-  g->bytes = g->off_acc + g->slots * g->R * g->D4 * 4;
+  g->bytes = g->cluster ? 0 : g->off_acc + g->slots * g->R * g->D4 * 4;
   return FE_STATUS_OK;
 }
 
@@ -97,11 +129,11 @@ int launch_dependent(Kern kern, dim3 grid, dim3 block, cudaStream_t stream, cons
   return FE_STATUS_OK;
 }
 
-template <bool BF16, int DP, bool DUAL>
+template <bool BF16, int DP, bool DUAL, bool CLUSTER>
 int launch_tree(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn, const CUtensorMap& tvn,
                 const fe::TreeParams& p, cudaStream_t stream) {
   using C = fe::TreeCfg<DP, DUAL>;
-  auto kern = fe::fe_tree_kernel<BF16, DP, DUAL>;
+  auto kern = fe::fe_tree_kernel<BF16, DP, DUAL, CLUSTER>;
   int rc = set_smem(kern, C::SMEM);
   if (rc) return rc;
   // setmaxnreg draws on the launch's own registers (see launch_fwd).
@@ -117,12 +149,30 @@ int launch_tree(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
   if (regs < fe::FWD_REGS_NEEDED)
     return fail(FE_STATUS_UNSUPPORTED, "tree attention kernel compiled with %d registers/thread, needs %d", regs,
                 fe::FWD_REGS_NEEDED);
+  const int64_t items = (int64_t)p.B * p.Hkv * p.MT;
+  if constexpr (CLUSTER) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)(items * fe::TREE_CLUSTER));
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = fe::TREE_CLUSTER;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, tkn, tvn, p);
+    if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
+    return FE_STATUS_OK;
+  }
   kern<<<dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, stream>>>(tq, tk, tv, tkn, tvn, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
   // Warps that share a row's partials: one per two partials (about ctas / items
   // of them), as long as the blocks are all resident at once (two an SM).
-  const int64_t items = (int64_t)p.B * p.Hkv * p.MT;
   const int64_t groups = (p.D4 / 4 + fe::TREE_JOIN_QUADS - 1) / fe::TREE_JOIN_QUADS, pairs = p.R * groups;
   auto blocks = [&](int splits) {
     const int64_t per_block = 32 * (fe::TREE_JOIN_WARPS / splits);
@@ -135,16 +185,36 @@ int launch_tree(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
 }
 
 template <bool BF16>
-int launch_tree_dim(int dp, bool dual, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn,
-                    const CUtensorMap& tvn, const fe::TreeParams& p, cudaStream_t s) {
-  if (dp == 64) return dual ? launch_tree<BF16, 64, true>(tq, tk, tv, tkn, tvn, p, s) : launch_tree<BF16, 64, false>(tq, tk, tv, tkn, tvn, p, s);
-  if (dp == 128) return dual ? launch_tree<BF16, 128, true>(tq, tk, tv, tkn, tvn, p, s) : launch_tree<BF16, 128, false>(tq, tk, tv, tkn, tvn, p, s);
-  return launch_tree<BF16, 256, false>(tq, tk, tv, tkn, tvn, p, s);
+int launch_tree_dim(int dp, const TreeGeometry& g, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                    const CUtensorMap& tkn, const CUtensorMap& tvn, const fe::TreeParams& p, cudaStream_t s) {
+  if (dp == 64)
+    return g.dual      ? launch_tree<BF16, 64, true, false>(tq, tk, tv, tkn, tvn, p, s)
+           : g.cluster ? launch_tree<BF16, 64, false, true>(tq, tk, tv, tkn, tvn, p, s)
+                       : launch_tree<BF16, 64, false, false>(tq, tk, tv, tkn, tvn, p, s);
+  if (dp == 128)
+    return g.dual      ? launch_tree<BF16, 128, true, false>(tq, tk, tv, tkn, tvn, p, s)
+           : g.cluster ? launch_tree<BF16, 128, false, true>(tq, tk, tv, tkn, tvn, p, s)
+                       : launch_tree<BF16, 128, false, false>(tq, tk, tv, tkn, tvn, p, s);
+  return g.cluster ? launch_tree<BF16, 256, false, true>(tq, tk, tv, tkn, tvn, p, s)
+                   : launch_tree<BF16, 256, false, false>(tq, tk, tv, tkn, tvn, p, s);
 }
 
 }  // namespace
 
 extern "C" {
+
+int fe_cache_prepare(fe_cache* cache) {
+  g_err[0] = 0;
+  int rc = check_cache(cache);
+  if (rc) return rc;
+  cache->maps_of = 0;
+  CUtensorMap tk, tv;
+  if ((rc = cache_maps(cache, &tk, &tv))) return rc;
+  memcpy(cache->map_k, &tk, sizeof(tk));
+  memcpy(cache->map_v, &tv, sizeof(tv));
+  cache->maps_of = layout_hash(cache);
+  return FE_STATUS_OK;
+}
 
 int64_t fe_tree_workspace_bytes(const fe_cache* cache, int64_t q_heads, int64_t drafts) {
   g_err[0] = 0;
@@ -165,7 +235,7 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   int rc = check_cache(cache);
   if (rc) return rc;
   if ((rc = check_drafts(cache, q_heads, drafts))) return rc;
-  if (!q || !k_new || !v_new || !out || !lse || !workspace || !q_strides || !k_new_strides || !v_new_strides)
+  if (!q || !k_new || !v_new || !out || !lse || !q_strides || !k_new_strides || !v_new_strides)
     return fail(FE_STATUS_INVALID, "null pointer");
   if (!std::isfinite(scale)) return fail(FE_STATUS_INVALID, "scale must be finite");
   if (q_strides[3] != 1) return fail(FE_STATUS_UNSUPPORTED, "q: channel stride must be 1");
@@ -177,12 +247,11 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   const int64_t B = cache->batch, H = cache->kv_heads, D = cache->channels;
   TreeGeometry g;
   if ((rc = tree_geometry(B, q_heads, H, drafts, cache->capacity, D, sm_count(dev), &g))) return rc;
-  if (workspace_bytes < g.bytes)
+  if (workspace_bytes < g.bytes || (g.bytes > 0 && !workspace))
     return fail(FE_STATUS_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)g.bytes);
   CUtensorMap tq, tk, tv, tkn, tvn;
   if ((rc = make_map(&tq, q, q_strides, B, q_heads, drafts, D, cache->dtype, "q", (int)drafts, g.heads))) return rc;
-  if ((rc = make_map(&tk, cache->k, cache->k_strides, B, H, cache->capacity, D, cache->dtype, "cache k"))) return rc;
-  if ((rc = make_map(&tv, cache->v, cache->v_strides, B, H, cache->capacity, D, cache->dtype, "cache v"))) return rc;
+  if ((rc = cache_maps(cache, &tk, &tv))) return rc;
   if ((rc = make_map(&tkn, k_new, k_new_strides, B, H, drafts, D, cache->dtype, "k_new"))) return rc;
   if ((rc = make_map(&tvn, v_new, v_new_strides, B, H, drafts, D, cache->dtype, "v_new"))) return rc;
   fe::TreeParams p;
@@ -218,8 +287,8 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   p.timeout_ns = (uint64_t)g_watchdog_ns;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int dp = padded_dim(D);
-  return cache->dtype == FE_DTYPE_BF16 ? launch_tree_dim<true>(dp, g.dual, tq, tk, tv, tkn, tvn, p, s)
-                                       : launch_tree_dim<false>(dp, g.dual, tq, tk, tv, tkn, tvn, p, s);
+  return cache->dtype == FE_DTYPE_BF16 ? launch_tree_dim<true>(dp, g, tq, tk, tv, tkn, tvn, p, s)
+                                       : launch_tree_dim<false>(dp, g, tq, tk, tv, tkn, tvn, p, s);
 }
 
 }  // extern "C"
@@ -247,10 +316,14 @@ int check_bookkeeping(const fe_cache* c, const fe_cache* out) {
   return FE_STATUS_OK;
 }
 
-int64_t commit_workspace(const fe_cache* c, int64_t drafts, int64_t* off_lengths) {
+// Drafts' weights between launches, and (in place) the new lengths.
+int64_t commit_workspace(const fe_cache* c, bool in_place, int64_t q_heads, int64_t drafts, int64_t max_accepted,
+                         int64_t* off_lengths) {
   const int64_t nbh = c->batch * c->kv_heads;
-  *off_lengths = round_up(nbh * drafts * 4, 256);
-  return *off_lengths + nbh * 4;
+  const int64_t rows = c->channels <= 128 ? fe::CommitCfg<128>::ROWS : fe::CommitCfg<256>::ROWS;
+  const bool launches = q_heads / c->kv_heads * max_accepted > rows;
+  *off_lengths = launches ? round_up(nbh * drafts * 4, 256) : 0;
+  return *off_lengths + (in_place ? nbh * 4 : 0);
 }
 
 template <bool BF16, int DP>
@@ -274,15 +347,12 @@ int launch_commit(const CUtensorMap& tk, const CUtensorMap& tkn, fe::CommitParam
 
 extern "C" {
 
-int64_t fe_commit_workspace_bytes(const fe_cache* cache, int64_t drafts) {
+int64_t fe_commit_workspace_bytes(const fe_cache* cache, const fe_cache* out, int64_t q_heads, int64_t drafts,
+                                  int64_t max_accepted) {
   g_err[0] = 0;
-  if (check_cache(cache)) return -1;
-  if (drafts < 1 || drafts > kMaxDrafts) {
-    fail(FE_STATUS_INVALID, "drafts out of range");
-    return -1;
-  }
+  if (check_bookkeeping(cache, out) || check_drafts(cache, q_heads, drafts)) return -1;
   int64_t off;
-  return commit_workspace(cache, drafts, &off);
+  return commit_workspace(cache, cache->mass == out->mass, q_heads, drafts, max_accepted, &off);
 }
 
 int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, const int64_t* q_strides,
@@ -296,7 +366,7 @@ int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, 
   if ((rc = check_drafts(cache, q_heads, drafts))) return rc;
   if (max_accepted < 1 || max_accepted > fe::COMMIT_MAX_ACCEPTED)
     return fail(FE_STATUS_INVALID, "max_accepted must be in [1, %d]", fe::COMMIT_MAX_ACCEPTED);
-  if (!q || !k_new || !v_new || !lse || !accepted || !new_positions || !workspace || !q_strides || !k_new_strides ||
+  if (!q || !k_new || !v_new || !lse || !accepted || !new_positions || !q_strides || !k_new_strides ||
       !v_new_strides)
     return fail(FE_STATUS_INVALID, "null pointer");
   if (!std::isfinite(scale)) return fail(FE_STATUS_INVALID, "scale must be finite");
@@ -306,8 +376,8 @@ int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, 
   if (tree_batch_stride < 0) return fail(FE_STATUS_INVALID, "tree_batch_stride must be nonnegative");
   const int64_t B = cache->batch, H = cache->kv_heads, D = cache->channels;
   int64_t off_lengths;
-  if (workspace_bytes < commit_workspace(cache, drafts, &off_lengths))
-    return fail(FE_STATUS_INVALID, "workspace too small");
+  const int64_t need = commit_workspace(cache, cache->mass == out->mass, q_heads, drafts, max_accepted, &off_lengths);
+  if (workspace_bytes < need || (need > 0 && !workspace)) return fail(FE_STATUS_INVALID, "workspace too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 4) return fail(FE_STATUS_UNSUPPORTED, "workspace must be 4-byte aligned");
   if (cache->mass == out->mass && !cache->sync) return fail(FE_STATUS_INVALID, "the cache has no sync word");
   const int64_t units = B * H * ((cache->capacity + fe::DEC_TILE - 1) / fe::DEC_TILE + 1);
@@ -315,7 +385,7 @@ int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, 
   int dev = 0;
   if ((rc = enter(cache->k, stream, &dev))) return rc;
   CUtensorMap tk, tkn;
-  if ((rc = make_map(&tk, cache->k, cache->k_strides, B, H, cache->capacity, D, cache->dtype, "cache k"))) return rc;
+  if ((rc = cache_maps(cache, &tk, nullptr))) return rc;
   if ((rc = make_map(&tkn, k_new, k_new_strides, B, H, drafts, D, cache->dtype, "k_new"))) return rc;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   fe::CommitParams p;

@@ -15,7 +15,10 @@
 // Work: all rows' key tiles laid end to end, one equal run per SM
 // (fe_decode.cuh), the last tile of a row being its drafts.  Each run leaves
 // an unnormalised partial (O, m, l) per row it touched; fe_tree_join_kernel
-// joins them in a fixed order (no atomics, bitwise reproducible).
+// joins them in a fixed order (no atomics, bitwise reproducible).  Few short
+// rows (a decode step over compacted caches) are latency instead: there a
+// cluster of eight CTAs has a row and joins through distributed shared memory,
+// in one launch (CLUSTER; 12.4 -> XX us for 4 rows of 2048).
 //
 // Roles (384 threads): warps 0-3 and 4-7 are two softmax warpgroups, warp 8
 // issues TMA, warp 9 tcgen05.mma.  Up to 128 rows (SPLIT) both warpgroups
@@ -24,6 +27,8 @@
 // (DUAL) they hold two query tiles and both use every key tile.  Heads of more
 // than 128 channels run one warpgroup (a 256-column O leaves no room for two).
 #pragma once
+
+#include <cooperative_groups.h>
 
 #include "fe_decode.cuh"
 #include "fe_forward.cuh"
@@ -184,7 +189,64 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
   return (w & E) == E || ((w >> 16) & E) == E;
 }
 
-template <bool BF16, int DP, bool DUAL>
+constexpr int TREE_CLUSTER = 8;
+
+// Running combination of partials of one row: four channels per quad.
+template <int Q>
+struct TreeMerge {
+  float m, l;
+  float4 a[Q];
+  __device__ __forceinline__ void init() {
+    m = TREE_M0;
+    l = 0.f;
+#pragma unroll
+    for (int j = 0; j < Q; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ void add(float2 st, const float4 (&v)[Q]) {
+    if (st.y == 0.f) return;  // this part saw no key of the row: its O may not have been written
+    const float mn = fmaxf(m, st.x);
+    const float f = exp2f(m - mn), g = exp2f(st.x - mn);
+    m = mn;
+    l = l * f + st.y * g;
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+      a[j].x = a[j].x * f + v[j].x * g;
+      a[j].y = a[j].y * f + v[j].y * g;
+      a[j].z = a[j].z * f + v[j].z * g;
+      a[j].w = a[j].w * f + v[j].w * g;
+    }
+  }
+  // Writes the row's channels [quad0*4, ...) and, with the first of them, its lse.
+  template <bool BF16>
+  __device__ __forceinline__ void store(const TreeParams& p, int64_t orow, int quad0) const {
+    const bool none = l == 0.f;
+    const float inv = none ? 0.f : 1.0f / l;
+    uint16_t* out = p.out + orow * p.D;
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+      const int c = (quad0 + j) * 4;
+      if (c >= p.D) continue;
+      const uint32_t lo = pack2<BF16>(a[j].x * inv, a[j].y * inv), hi = pack2<BF16>(a[j].z * inv, a[j].w * inv);
+      if ((p.D & 3) == 0) {
+        *reinterpret_cast<uint2*>(out + c) = make_uint2(lo, hi);
+      } else {
+        const uint16_t w[4] = {static_cast<uint16_t>(lo), static_cast<uint16_t>(lo >> 16), static_cast<uint16_t>(hi),
+                               static_cast<uint16_t>(hi >> 16)};
+        for (int i = 0; i < 4 && c + i < p.D; ++i) out[c + i] = w[i];
+      }
+    }
+    if (quad0 == 0) p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  }
+};
+
+// All threads of the cluster, each warp converged; the roles meet here from
+// different places.
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <bool BF16, int DP, bool DUAL, bool CLUSTER>
 __global__ void __launch_bounds__(384, 1)
     fe_tree_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv,
@@ -215,7 +277,7 @@ __global__ void __launch_bounds__(384, 1)
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
 
-  pdl_launch_dependents();
+  if constexpr (!CLUSTER) pdl_launch_dependents();
   if (threadIdx.x == 256) {
     tma_prefetch_desc(&tq);
     tma_prefetch_desc(&tk);
@@ -249,8 +311,24 @@ __global__ void __launch_bounds__(384, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  // Ends with a block barrier, which also publishes the barriers and TMEM.
-  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, p.MT, TREE_EXTRA, blockIdx.x, p.nctas, scratch);
+  DecWalk walk;
+  if constexpr (CLUSTER) {
+    // A CTA of the cluster has an eighth of one item's tiles.
+    const int item = blockIdx.x / TREE_CLUSTER, rank = blockIdx.x % TREE_CLUSTER;
+    walk.lengths = p.lengths;
+    walk.capacity = p.capacity;
+    walk.mts = p.MT;
+    walk.extra = 0;
+    walk.bh = item / p.MT;
+    const int tiles = (cache_length(p.lengths, walk.bh, p.capacity) + DEC_TILE - 1) / DEC_TILE + 1;
+    const int share = (tiles + TREE_CLUSTER - 1) / TREE_CLUSTER, j0 = min(rank * share, tiles);
+    walk.left = min(share, tiles - j0);
+    walk.unit = (item - walk.bh * p.MT) * tiles + j0;
+    __syncthreads();
+  } else {
+    // Ends with a block barrier, which also publishes the barriers and TMEM.
+    walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, p.MT, TREE_EXTRA, blockIdx.x, p.nctas, scratch);
+  }
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   const uint64_t TO = p.timeout_ns;
@@ -389,6 +467,10 @@ __global__ void __launch_bounds__(384, 1)
         mbar_wait_inflight(drain, 0, TO);
       }
     }
+    if constexpr (CLUSTER) {
+      cluster_barrier();
+      cluster_barrier();
+    }
   } else {
     setmaxnreg_inc<FWD_REGS_HIGH>();
     // ------------------------------------------------------------- softmax --
@@ -401,6 +483,10 @@ __global__ void __launch_bounds__(384, 1)
       const float sc = p.sc;
       const bool sc_pos = sc > 0.f;
       const float sce = sc_pos ? sc : 1.0f;
+      // CLUSTER: the partial stays in shared memory, in the place of the tiles
+      // (every load has landed and every product has read them by then).
+      float4* s_part = reinterpret_cast<float4*>(smem);
+      float2* s_part_stats = reinterpret_cast<float2*>(smem + C::OFF_BAR - 128 * 8);
       bool ok = true;
       uint32_t it0 = 0, nseg = 0, ns = 0;  // key tiles before, segments, S tiles of this group
       for (; walk.next(sg); ++nseg) {
@@ -494,7 +580,7 @@ __global__ void __launch_bounds__(384, 1)
         tc_fence_after();
         // ---- result of this run for the row: a partial, or the row itself
         // when the run has all of its tiles
-        const bool whole = sg.j0 == 0 && sg.j1 == sg.tiles;
+        const bool whole = !CLUSTER && sg.j0 == 0 && sg.j1 == sg.tiles;
         const float nan = __int_as_float(0x7fffffff);
         float f0 = 1.f, f1 = 0.f;  // weights of O of this group's lanes, and (SPLIT) of the other warpgroup's
         if (!ok) m_used = l = nan;  // aborted (watchdog): everything below becomes NaN
@@ -519,7 +605,8 @@ __global__ void __launch_bounds__(384, 1)
         const bool two = C::SPLIT && ntile > 1;
         const int64_t slot = static_cast<int64_t>(sg.bh) * p.MT + sg.mt + blockIdx.x;
         const int64_t orow = static_cast<int64_t>(sg.bh) * p.M + row;
-        float4* dst = p.acc + slot * p.R * (p.D4 / 4) + pr;
+        float4* dst = CLUSTER ? s_part + pr : p.acc + slot * p.R * (p.D4 / 4) + pr;
+        float2* dst_stats = CLUSTER ? s_part_stats : p.stats + slot * p.R;
         uint16_t* out = p.out + orow * p.D;
         // Special rows are added in memory, so such a run's sum goes through it.
         const bool special_rows = has_drafts && (spec[0] | spec[1] | spec[2] | spec[3]) != 0u;
@@ -527,7 +614,7 @@ __global__ void __launch_bounds__(384, 1)
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         if (live && (!C::SPLIT || t == 0)) {
           if (whole) p.lse[orow] = l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
-          else p.stats[slot * p.R + pr] = make_float2(m_used, l);
+          else dst_stats[pr] = make_float2(m_used, l);
         }
         if (warp_live) {
           constexpr int CB = C::SPLIT ? DP / 2 : DP;
@@ -580,6 +667,35 @@ __global__ void __launch_bounds__(384, 1)
         if constexpr (C::SPLIT) named_bar_sync(3, 256);  // both are done with both O tiles
         it0 += ntile;
       }
+      if constexpr (CLUSTER) {
+        if (nseg == 0 && t == 0) s_part_stats[r] = make_float2(TREE_M0, 0.f);
+        cluster_barrier();
+        // Every CTA joins an eighth of the item's rows and channels.
+        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        const int item = blockIdx.x / TREE_CLUSTER, rank = blockIdx.x % TREE_CLUSTER;
+        const int bh = item / p.MT, mt = item - bh * p.MT;
+        const int rows = min(p.M - mt * p.tile_rows, p.tile_rows), pairs = rows * (p.D4 / 4);
+        const int share = (pairs + TREE_CLUSTER - 1) / TREE_CLUSTER, end = min(pairs, (rank + 1) * share);
+        for (int i = rank * share + t * 128 + r; i < end; i += NG * 128) {
+          const int quad = i / rows, rr = i - quad * rows;
+          float2 st[TREE_CLUSTER];
+          float4 v[TREE_CLUSTER][1];
+#pragma unroll
+          for (int c = 0; c < TREE_CLUSTER; ++c) {
+            st[c] = *cluster.map_shared_rank(s_part_stats + rr, c);
+            v[c][0] = *cluster.map_shared_rank(s_part + quad * p.R + rr, c);
+          }
+          TreeMerge<1> sum;
+          sum.init();
+#pragma unroll
+          for (int c = 0; c < TREE_CLUSTER; ++c) sum.add(st[c], v[c]);
+          sum.template store<BF16>(p, static_cast<int64_t>(bh) * p.M + mt * p.tile_rows + rr, quad);
+        }
+        cluster_barrier();  // nobody leaves while a neighbour reads its partial
+      }
+    } else if constexpr (CLUSTER) {
+      cluster_barrier();
+      cluster_barrier();
     }
   }
 
@@ -634,24 +750,8 @@ __global__ void __launch_bounds__(TREE_JOIN_THREADS)
   const float2* st_row = p.stats + slot0 * p.R + r;
   const float4* acc_row = p.acc + slot0 * p.R * quads + static_cast<int64_t>(quad0) * p.R + r;
   const int64_t acc_step = static_cast<int64_t>(p.R) * quads;
-  float m = TREE_M0, l = 0.f;
-  float4 a[Q];
-#pragma unroll
-  for (int j = 0; j < Q; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto merge = [&](float2 st, const float4 (&v)[Q]) {
-    if (st.y == 0.f) return;  // this run saw no key of the row: its O was not written
-    const float mn = fmaxf(m, st.x);
-    const float f = exp2f(m - mn), g = exp2f(st.x - mn);
-    m = mn;
-    l = l * f + st.y * g;
-#pragma unroll
-    for (int j = 0; j < Q; ++j) {
-      a[j].x = a[j].x * f + v[j].x * g;
-      a[j].y = a[j].y * f + v[j].y * g;
-      a[j].z = a[j].z * f + v[j].z * g;
-      a[j].w = a[j].w * f + v[j].w * g;
-    }
-  };
+  TreeMerge<Q> sum;
+  sum.init();
   if (live) {
     constexpr int U = 3;
     for (int i0 = split; i0 < n; i0 += splits * U) {
@@ -669,41 +769,23 @@ __global__ void __launch_bounds__(TREE_JOIN_THREADS)
         }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) merge(st[u], v[u]);
+      for (int u = 0; u < U; ++u) sum.add(st[u], v[u]);
     }
   }
   if (splits > 1) {
-    s_ml[warp][lane] = make_float2(m, l);
+    s_ml[warp][lane] = make_float2(sum.m, sum.l);
 #pragma unroll
-    for (int j = 0; j < Q; ++j) s_acc[warp][j][lane] = a[j];
+    for (int j = 0; j < Q; ++j) s_acc[warp][j][lane] = sum.a[j];
     __syncthreads();
     if (split != 0) return;
     for (int w = 1; w < splits; ++w) {
       float4 v[Q];
 #pragma unroll
       for (int j = 0; j < Q; ++j) v[j] = s_acc[warp + w][j][lane];
-      merge(s_ml[warp + w][lane], v);
+      sum.add(s_ml[warp + w][lane], v);
     }
   }
-  if (!live) return;
-  const bool none = l == 0.f;
-  const float inv = none ? 0.f : 1.0f / l;
-  const int64_t orow = static_cast<int64_t>(bh) * p.M + mt * rows_per_item + r;
-  uint16_t* out = p.out + orow * p.D;
-#pragma unroll
-  for (int j = 0; j < Q; ++j) {
-    const int c = (quad0 + j) * 4;
-    if (c >= p.D) continue;
-    const uint32_t lo = pack2<BF16>(a[j].x * inv, a[j].y * inv), hi = pack2<BF16>(a[j].z * inv, a[j].w * inv);
-    if ((p.D & 3) == 0) {
-      *reinterpret_cast<uint2*>(out + c) = make_uint2(lo, hi);
-    } else {
-      const uint16_t w[4] = {static_cast<uint16_t>(lo), static_cast<uint16_t>(lo >> 16), static_cast<uint16_t>(hi),
-                             static_cast<uint16_t>(hi >> 16)};
-      for (int i = 0; i < 4 && c + i < p.D; ++i) out[c + i] = w[i];
-    }
-  }
-  if (quad0 == 0) p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  if (live) sum.template store<BF16>(p, static_cast<int64_t>(bh) * p.M + mt * rows_per_item + r, quad0);
 }
 
 }  // namespace fe

@@ -43,7 +43,8 @@ class Cache(ctypes.Structure):
     """fe_cache of include/flash_evict.h."""
     _fields_ = [("k", _VP), ("v", _VP), ("k_strides", _I64 * 4), ("v_strides", _I64 * 4), ("mass", _VP),
                 ("norms", _VP), ("positions", _VP), ("lengths", _VP), ("sync", _VP), ("batch", _I64), ("kv_heads", _I64),
-                ("capacity", _I64), ("channels", _I64), ("dtype", _INT)]
+                ("capacity", _I64), ("channels", _I64), ("dtype", _INT), ("maps_of", ctypes.c_uint64),
+                ("map_k", ctypes.c_uint64 * 16), ("map_v", ctypes.c_uint64 * 16)]
 
 
 _CACHEP = ctypes.POINTER(Cache)
@@ -72,10 +73,11 @@ SIGNATURES = {
                               _I64, _VP]),
     "fe_evict_noalloc": (_INT, [_VP, _I64P, _VP, _I64P, _VP, _I64P, _VP, _VP, _VP, _VP, _I64, _I64, _I64,
                                 _I64, _I64, _INT, _INT, _F32, _F32, _I64, _INT, _I64, _I64, _I64, _VP]),
+    "fe_cache_prepare": (_INT, [_CACHEP]),
     "fe_tree_workspace_bytes": (_I64, [_CACHEP, _I64, _I64]),
     "fe_tree_attention": (_INT, [_CACHEP, _VP, _I64P, _VP, _I64P, _VP, _I64P, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64,
                                  _F32, _VP]),
-    "fe_commit_workspace_bytes": (_I64, [_CACHEP, _I64]),
+    "fe_commit_workspace_bytes": (_I64, [_CACHEP, _CACHEP, _I64, _I64, _I64]),
     "fe_commit_tokens": (_INT, [_CACHEP, _CACHEP, _VP, _I64P, _VP, _I64P, _VP, _I64P, _VP, _I64, _VP, _VP, _I64, _VP, _VP,
                                 _I64, _I64, _I64, _F32, _F32, _VP]),
     "fe_evict_workspace_bytes": (_I64, [_CACHEP, _I64]),

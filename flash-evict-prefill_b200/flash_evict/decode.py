@@ -45,7 +45,7 @@ class KVCache:
     copied, and cannot be replaced: update them in place.
     """
 
-    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "device", "dtype", "_sync", "_c", "_ref", "_device_index")
+    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "device", "dtype", "_sync", "_sizes", "_c", "_ref", "_device_index")
 
     def __init__(self, k, v, lengths, mass=None, positions=None, norms=None):
         if k.ndim != 4 or k.shape != v.shape or k.numel() == 0 or k.shape[-1] > 256:
@@ -70,6 +70,8 @@ class KVCache:
         init(self, "_c", _lib.Cache(k.data_ptr(), v.data_ptr(), k.stride(), v.stride(), ptr(mass), ptr(norms), ptr(positions),
                                     lengths.data_ptr(), ptr(self._sync), b, h, c, d, _DTYPES[k.dtype]))
         init(self, "_ref", ctypes.byref(self._c))
+        init(self, "_sizes", {})  # workspace bytes by the calls' shapes
+        _lib.check(_lib.load().fe_cache_prepare(self._ref))
         init(self, "device", k.device)
         init(self, "dtype", k.dtype)
         init(self, "_device_index", k.device.index)
@@ -125,6 +127,20 @@ def _readable(t):
         t = _tma_view(t)
         st = t.stride()
     return t, _stride_array(st)
+
+
+def _workspace(cache, key, bytes_of, *args):
+    # (size, tensor, pointer) of a call's workspace; its size depends on the shapes alone.
+    size = cache._sizes.get(key)
+    if size is None:
+        size = bytes_of(*args)
+        if size < 0:
+            _lib.check(_lib.STATUS_UNSUPPORTED)
+        cache._sizes[key] = size
+    if size == 0:
+        return 0, None, None
+    tensor = torch.empty(size, dtype=torch.uint8, device=cache.device)
+    return size, tensor, tensor.data_ptr()
 
 
 def _call(fn, device_index, *args):
@@ -183,18 +199,14 @@ def tree_attention(q, k_new, v_new, cache, *, tree=None, scale=None):
     tree, tree_stride, scale = _check_drafts(q, k_new, v_new, cache, tree, scale)
     b, hq, t, d = q.shape
     lib = _lib.load()
-    size = lib.fe_tree_workspace_bytes(cache._ref, hq, t)
-    if size < 0:
-        _lib.check(_lib.STATUS_UNSUPPORTED)
+    size, workspace, pointer = _workspace(cache, (hq, t), lib.fe_tree_workspace_bytes, cache._ref, hq, t)
     out = q.new_empty((b, hq, t, d))
     lse = torch.empty((b, hq, t), dtype=torch.float32, device=q.device)
-    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
     q, qs = _readable(q)
     k_new, ks = _readable(k_new)
     v_new, vs = _readable(v_new)
     _call(lib.fe_tree_attention, cache._device_index, cache._ref, q.data_ptr(), qs, k_new.data_ptr(), ks, v_new.data_ptr(), vs,
-          None if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(), lse.data_ptr(), workspace.data_ptr(), size, hq,
-          t, scale)
+          None if tree is None else tree.data_ptr(), tree_stride, out.data_ptr(), lse.data_ptr(), pointer, size, hq, t, scale)
     return out, lse
 
 
@@ -248,8 +260,8 @@ def commit_tokens(cache, q, k_new, v_new, lse, accepted, positions, *, tree=None
     if not math.isfinite(recency_decay) or recency_decay < 0:
         raise ValueError("recency_decay must be finite and nonnegative")
     lib = _lib.load()
-    size = lib.fe_commit_workspace_bytes(cache._ref, t)
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    a = accepted.shape[1]
+    size, workspace, pointer = _workspace(cache, (hq, t, a, out is cache), lib.fe_commit_workspace_bytes, cache._ref, out._ref, hq, t, a)
     q, qs = _readable(q)
     k_new, ks = _readable(k_new)
     v_new, vs = _readable(v_new)
@@ -257,7 +269,7 @@ def commit_tokens(cache, q, k_new, v_new, lse, accepted, positions, *, tree=None
         lse, accepted, positions = lse.contiguous(), accepted.contiguous(), positions.contiguous()
     _call(lib.fe_commit_tokens, cache._device_index, cache._ref, out._ref, q.data_ptr(), qs, k_new.data_ptr(), ks,
           v_new.data_ptr(), vs, None if tree is None else tree.data_ptr(), tree_stride,
-          lse.data_ptr(), accepted.data_ptr(), accepted.shape[1], positions.data_ptr(), workspace.data_ptr(), size, hq, t,
+          lse.data_ptr(), accepted.data_ptr(), a, positions.data_ptr(), pointer, size, hq, t,
           scale, recency_decay)
     return out
 
@@ -278,7 +290,6 @@ def evict_tokens(cache, budget, *, recent=0, out=None):
     if isinstance(recent, bool) or not isinstance(recent, int) or not 0 <= recent <= budget:
         raise ValueError("recent must be an integer in [0, budget]")
     lib = _lib.load()
-    size = lib.fe_evict_workspace_bytes(cache._ref, budget)
-    workspace = torch.empty(size, dtype=torch.uint8, device=cache.device)
-    _call(lib.fe_evict_tokens, cache._device_index, cache._ref, out._ref, budget, recent, workspace.data_ptr(), size)
+    size, workspace, pointer = _workspace(cache, budget, lib.fe_evict_workspace_bytes, cache._ref, budget)
+    _call(lib.fe_evict_tokens, cache._device_index, cache._ref, out._ref, budget, recent, pointer, size)
     return out

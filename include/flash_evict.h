@@ -272,7 +272,14 @@ typedef struct fe_cache {
   int32_t* sync;      /* one word, zero, for fe_commit_tokens in place (it is zero again after) */
   int64_t batch, kv_heads, capacity, channels;
   int dtype;
+  /* Written by fe_cache_prepare; zero-initialise. */
+  uint64_t maps_of;
+  uint64_t map_k[16], map_v[16];
 } fe_cache;
+
+/* Optional: make the cache's tensor maps once instead of in every call.  The
+ * calls use them as long as the fields above are what they were then. */
+FE_API int fe_cache_prepare(fe_cache* cache);
 
 /* Attention of `drafts` (1..128) drafted tokens per sequence over the cache and
  * over each other: draft t sees every cached token of its row and the drafts j
@@ -283,8 +290,9 @@ typedef struct fe_cache {
  *   lse: FP32 [batch, q_heads, drafts], the natural logarithm of the sum of
  *   exp(scale * q.k) (-inf, with out 0, for a row that sees nothing).
  * q, k_new and v_new follow the layout rules above.
- * workspace: fe_tree_workspace_bytes() bytes on the cache's device, 256-byte
- * aligned, contents irrelevant.  Two launches; bitwise reproducible. */
+ * workspace: fe_tree_workspace_bytes() bytes (may be 0) on the cache's device,
+ * 256-byte aligned, contents irrelevant.  One or two launches; bitwise
+ * reproducible. */
 FE_API int64_t fe_tree_workspace_bytes(const fe_cache* cache, int64_t q_heads, int64_t drafts);
 FE_API int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_strides, const void* k_new,
                              const int64_t* k_new_strides, const void* v_new, const int64_t* v_new_strides,
@@ -308,7 +316,8 @@ FE_API int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t
  * k and v whose arrays are all others (then `cache` still describes the tokens
  * before the call); only slots below the new lengths are written.  Each element
  * is written once in a fixed order (no atomics, bitwise reproducible). */
-FE_API int64_t fe_commit_workspace_bytes(const fe_cache* cache, int64_t drafts);
+FE_API int64_t fe_commit_workspace_bytes(const fe_cache* cache, const fe_cache* out, int64_t q_heads, int64_t drafts,
+                                         int64_t max_accepted);
 FE_API int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, const int64_t* q_strides,
                             const void* k_new, const int64_t* k_new_strides, const void* v_new,
                             const int64_t* v_new_strides, const uint8_t* tree, int64_t tree_batch_stride,

@@ -45,6 +45,7 @@ def test_c_abi_refusals_without_a_gpu():
     assert lib.fe_tree_workspace_bytes(ctypes.byref(c_cache()), 4, 129) == -1
 
     def commit(cache, out, accepted=1, decay=0.0, size=1 << 20):
+        # (in place: needs a workspace for the new lengths)
         return lib.fe_commit_tokens(ctypes.byref(cache), ctypes.byref(out), fake, st, fake, st, fake, st, None, 0, fake, fake, accepted,
                                     fake, fake, size, 4, 2, 0.1, decay, None)
 
