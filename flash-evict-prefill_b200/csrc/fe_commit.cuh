@@ -68,9 +68,14 @@ struct CommitParams {
   int rows_vec;        // K/V rows can be moved 16 bytes at a time
   float sc;            // scale * log2(e)
   double decay_log2;
-  int q_vec;
+  int q_vec, tree_vec; // query rows, mask rows can be read 16 bytes at a time
   uint64_t timeout_ns;
 };
+
+// Registers: launched at 96 a thread (640 threads); the control warpgroup drops
+// to 64 and the four that reduce rise to 104 (4*128*104 + 128*64 = 640*96).
+constexpr uint32_t COMMIT_REGS_HIGH = 104, COMMIT_REGS_LOW = 64;
+constexpr int COMMIT_REGS_NEEDED = (4 * 128 * 104 + 128 * 64) / 640;
 
 template <int DP>
 struct CommitCfg {
@@ -85,8 +90,8 @@ struct CommitCfg {
   static constexpr int OFF_BIAS = OFF_K + STAGES * TILE;
   static constexpr int OFF_MASK = OFF_BIAS + ROWS * 4;                       // uint32[128][4]
   static constexpr int OFF_LIST = OFF_MASK + COMMIT_MAX_ACCEPTED * 16;      // int[128]
-  static constexpr int OFF_COL = OFF_LIST + COMMIT_MAX_ACCEPTED * 4;        // uint8[ROWS]
-  static constexpr int OFF_NEW = OFF_COL + ROWS;                            // float[2][128]: weights of new tokens
+  static constexpr int OFF_COL = OFF_LIST + COMMIT_MAX_ACCEPTED * 4;        // uint32[4][ROWS]: masks by column
+  static constexpr int OFF_NEW = OFF_COL + ROWS * 16;                       // float[2][128]: weights of new tokens
   static constexpr int OFF_APP = OFF_NEW + 2 * 128 * 4;                     // int list[128], float norm[128]
   static constexpr int OFF_BAR = OFF_APP + COMMIT_MAX_ACCEPTED * 8;
   // q_full, k_full[S], k_empty[S], s_full[WGS], s_free[WGS], drain, new_full[2], new_empty[2]
@@ -117,17 +122,19 @@ __device__ __forceinline__ int accepted_drafts(const int32_t* accepted, int A, i
 
 // Sum over `cols` (a multiple of 16, at most 128) query columns of one key's
 // S^T row of exp2(x * sc + bias); `release` is called once the row has been
-// read.  FULL: 128 columns, unrolled.  DRAFT: only columns whose query sees this
-// thread's draft (bit `bit` of word masks[col_query * 4]).
+// read.  FULL: 128 columns, unrolled.  DRAFT: only columns with bit `bit` of their word in
+// `masks` set.
 template <bool FULL, bool DRAFT, typename Release>
 __device__ __forceinline__ float commit_reduce(uint32_t tS, int cols, float sc, const float* bias, const uint32_t* masks,
-                                               const uint8_t* col_query, int bit, Release release) {
+                                               int bit, Release release) {
   const uint64_t sc2 = f2_pack(sc, sc);
   uint64_t acc2[4] = {0ull, 0ull, 0ull, 0ull};
   auto chunk = [&](int c0, const float (&x)[16]) {
 #pragma unroll
     for (int c4 = 0; c4 < 16; c4 += 4) {
       const float4 nb = *reinterpret_cast<const float4*>(bias + c0 + c4);
+      uint4 see = make_uint4(0u, 0u, 0u, 0u);
+      if (DRAFT) see = *reinterpret_cast<const uint4*>(masks + c0 + c4);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int c = c4 + 2 * u;
@@ -135,8 +142,8 @@ __device__ __forceinline__ float commit_reduce(uint32_t tS, int cols, float sc, 
         float a0, a1;
         f2_unpack(a2, a0, a1);
         if (DRAFT) {
-          a0 = ((masks[col_query[c0 + c] * 4] >> bit) & 1u) ? a0 : -INFINITY;
-          a1 = ((masks[col_query[c0 + c + 1] * 4] >> bit) & 1u) ? a1 : -INFINITY;
+          a0 = (((u == 0 ? see.x : see.z) >> bit) & 1u) ? a0 : -INFINITY;
+          a1 = (((u == 0 ? see.y : see.w) >> bit) & 1u) ? a1 : -INFINITY;
         }
         acc2[(c >> 1) & 3] = f2_add(acc2[(c >> 1) & 3], f2_pack(ex2_approx(a0), ex2_approx(a1)));
       }
@@ -171,12 +178,12 @@ __device__ __forceinline__ float commit_reduce(uint32_t tS, int cols, float sc, 
 }
 
 // Appends the K/V rows of cache row bh's accepted drafts, with their norms and
-// positions, by two warps (64 threads), eight rows a warp in flight.  The norms
+// positions, by two warps (64 threads), four rows a warp in flight.  The norms
 // are left in shared memory for the weights that follow.
 template <bool BF16>
 __device__ __forceinline__ void commit_append_rows(const CommitParams& p, int bh, int b, int h, int len, int fit,
                                                    const int* list, float* norms, int warp, int lane) {
-  constexpr int U = 8;
+  constexpr int U = 4;
   const int64_t base = static_cast<int64_t>(bh) * p.capacity;
   const uint16_t* kn = p.k_new + b * p.kn_sb + h * p.kn_sh;
   const uint16_t* vn = p.v_new + b * p.vn_sb + h * p.vn_sh;
@@ -248,7 +255,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
   float* sbias = reinterpret_cast<float*>(smem + C::OFF_BIAS);
   uint32_t* smask = reinterpret_cast<uint32_t*>(smem + C::OFF_MASK);
   int* slist = reinterpret_cast<int*>(smem + C::OFF_LIST);
-  uint8_t* scol = smem + C::OFF_COL;
+  uint32_t* scol = reinterpret_cast<uint32_t*>(smem + C::OFF_COL);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* k_full = q_full + 1;
   uint64_t* k_empty = k_full + C::STAGES;
@@ -301,6 +308,8 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
   DecSegment sg;
   auto rows_of = [&](int b, int n) { return min(max(n * p.G - p.row0, 0), C::ROWS); };
 
+  if (warp >= C::PRODUCER) {
+  setmaxnreg_dec<COMMIT_REGS_LOW>();
   if (warp == C::PRODUCER) {
     // ------------------------------------------------------------ producer --
     uint32_t it = 0;
@@ -384,7 +393,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
       umma_commit(drain);
       mbar_wait_inflight(drain, 0, TO);
     }
-  } else if (warp >= C::APPEND) {
+  } else {
     // -------------------------------------------------------------- append --
     const int w = warp - C::APPEND;
     int* list = reinterpret_cast<int*>(smem + C::OFF_APP);
@@ -419,7 +428,9 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         }
       }
     }
+  }
   } else {
+    setmaxnreg_inc<COMMIT_REGS_HIGH>();
     // ------------------------------------------------ reduce (thread = key) --
     const int wg = warp >> 2;
     const int kr = ((warp & 3) << 5) + static_cast<int>(lane);
@@ -469,7 +480,6 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         }
         for (int r = tid - QT; wg == C::WGS - 1 && r < padded; r += 128) {
           float bias = -INFINITY;  // padding, and rows that saw nothing, add 0
-          int query = 0;
           if (r < rows) {
             const int qi = (p.row0 + r) / p.G, g = p.row0 + r - qi * p.G;
             const float lse = __ldg(p.lse + (static_cast<int64_t>(b) * p.Hq + h * p.G + g) * p.T + slist[qi]);
@@ -477,25 +487,26 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
             // would be up to 1e-6 of a weight each.
             if (lse != -INFINITY)
               bias = static_cast<float>(-(p.decay_log2 * (n - 1 - qi) + static_cast<double>(lse) * 1.4426950408889634));
-            query = qi - i_first;
           }
-          scol[r] = static_cast<uint8_t>(query);
           sbias[r] = bias;
         }
         if (wg == C::WGS - 1 && sg.j1 == sg.tiles) {
-          // Which drafts each accepted query of this launch sees.
+          // Which drafts each accepted query of this launch sees, then by column.
           const int nq = (p.row0 + rows - 1) / p.G - i_first + 1;
           for (int i = tid - QT; i < nq * 4; i += 128) {
             const int t = slist[i_first + (i >> 2)], w = i & 3;
             const int cnt = min(max((p.tree == nullptr ? t + 1 : p.T) - 32 * w, 0), 32);
-            uint32_t bits = cnt == 32 ? 0xffffffffu : ((1u << cnt) - 1u);
-            if (p.tree != nullptr) {
-              const uint8_t* row = p.tree + b * p.tree_sb + static_cast<int64_t>(t) * p.T + 32 * w;
-              bits = 0u;
-#pragma unroll 8
-              for (int j = 0; j < cnt; ++j) bits |= (__ldg(row + j) != 0 ? 1u : 0u) << j;
-            }
-            smask[i] = bits;
+            smask[i] = p.tree == nullptr ? low_bits(cnt)
+                                         : mask_word(p.tree + b * p.tree_sb + static_cast<int64_t>(t) * p.T + 32 * w, cnt, p.tree_vec);
+          }
+          named_bar_sync(3, 128);
+          for (int r = tid - QT; r < padded; r += 128) {
+            const int i = r < rows ? (p.row0 + r) / p.G - i_first : 0;
+            const uint4 m = *reinterpret_cast<const uint4*>(smask + i * 4);
+            scol[r] = m.x;
+            scol[C::ROWS + r] = m.y;
+            scol[2 * C::ROWS + r] = m.z;
+            scol[3 * C::ROWS + r] = m.w;
           }
         }
         fence_proxy_async_smem();
@@ -536,11 +547,11 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
           };
           const float* bias = sbias + c * 128;
           if (drafts)
-            total += commit_reduce<false, true>(tS, cols, p.sc, bias, smask + (kr >> 5), scol + c * 128, kr & 31, release);
+            total += commit_reduce<false, true>(tS, cols, p.sc, bias, scol + (kr >> 5) * C::ROWS + c * 128, kr & 31, release);
           else if (cols == 128)
-            total += commit_reduce<true, false>(tS, cols, p.sc, bias, nullptr, nullptr, 0, release);
+            total += commit_reduce<true, false>(tS, cols, p.sc, bias, nullptr, 0, release);
           else
-            total += commit_reduce<false, false>(tS, cols, p.sc, bias, nullptr, nullptr, 0, release);
+            total += commit_reduce<false, false>(tS, cols, p.sc, bias, nullptr, 0, release);
         }
         // Aborted (watchdog): the sum is incomplete; store NaN.
         if (!ok) total = __int_as_float(0x7fffffff);

@@ -156,6 +156,32 @@ __device__ __forceinline__ uint4 load_row_chunk(const uint16_t* row, int chunk, 
   return v;
 }
 
+// Bits of up to 32 mask bytes (1 where nonzero).  vec: 16-byte aligned, n a
+// multiple of 16; otherwise all bytes are loaded before the first is used.
+__device__ __forceinline__ uint32_t mask_word(const uint8_t* row, int n, bool vec) {
+  uint32_t v = 0u;
+  if (vec) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (16 * u >= n) continue;
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(row) + u);
+      // Four mask bytes to four bits: 1 where nonzero, gathered by a multiply.
+      v |= ((__vsetgtu4(x.x, 0u) * 0x01020408u) >> 24) << (16 * u);
+      v |= ((__vsetgtu4(x.y, 0u) * 0x01020408u) >> 24) << (16 * u + 4);
+      v |= ((__vsetgtu4(x.z, 0u) * 0x01020408u) >> 24) << (16 * u + 8);
+      v |= ((__vsetgtu4(x.w, 0u) * 0x01020408u) >> 24) << (16 * u + 12);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < n) v |= (__ldg(row + j) != 0 ? 1u : 0u) << j;
+  }
+  return v;
+}
+
+// The lowest n bits, 0 <= n <= 32.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
 template <bool BF16>
 __device__ __forceinline__ float elem_to_float(uint16_t x) {
   if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(x) << 16);

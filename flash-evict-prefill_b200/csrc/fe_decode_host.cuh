@@ -75,6 +75,11 @@ bool rows_are_vectors(const void* p, const int64_t* s, int64_t batch, int64_t he
          (heads == 1 || s[1] % 8 == 0) && (tokens == 1 || s[2] % 8 == 0);
 }
 
+// Rows of [batch, drafts, drafts] mask bytes, the same.
+int mask_is_vectors(const void* tree, int64_t batch_stride, int64_t drafts) {
+  return tree && drafts % 16 == 0 && reinterpret_cast<uintptr_t>(tree) % 16 == 0 && batch_stride % 16 == 0;
+}
+
 int64_t round_up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 // Geometry of a tree-attention launch: a function of the shapes alone, so the
@@ -112,6 +117,22 @@ int tree_geometry(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t draf
   return FE_STATUS_OK;
 }
 
+// setmaxnreg draws on the registers a block was launched with (see launch_fwd).
+template <typename Kern>
+int check_regs(Kern kern, std::atomic<int>& checked, int needed, const char* what) {
+  int regs = checked.load(std::memory_order_relaxed);
+  if (regs == 0) {
+    cudaFuncAttributes fa;
+    cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
+    regs = fa.numRegs;
+    checked.store(regs, std::memory_order_relaxed);
+  }
+  if (regs < needed)
+    return fail(FE_STATUS_UNSUPPORTED, "%s kernel compiled with %d registers/thread, needs %d", what, regs, needed);
+  return FE_STATUS_OK;
+}
+
 template <typename Kern, typename... Args>
 int launch_dependent(Kern kern, dim3 grid, dim3 block, cudaStream_t stream, const char* what, Args... args) {
   cudaLaunchConfig_t cfg;
@@ -136,19 +157,8 @@ int launch_tree(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
   auto kern = fe::fe_tree_kernel<BF16, DP, DUAL, CLUSTER>;
   int rc = set_smem(kern, C::SMEM);
   if (rc) return rc;
-  // setmaxnreg draws on the launch's own registers (see launch_fwd).
   static std::atomic<int> checked_regs{0};
-  int regs = checked_regs.load(std::memory_order_relaxed);
-  if (regs == 0) {
-    cudaFuncAttributes fa;
-    cudaError_t e = cudaFuncGetAttributes(&fa, kern);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
-    regs = fa.numRegs;
-    checked_regs.store(regs, std::memory_order_relaxed);
-  }
-  if (regs < fe::FWD_REGS_NEEDED)
-    return fail(FE_STATUS_UNSUPPORTED, "tree attention kernel compiled with %d registers/thread, needs %d", regs,
-                fe::FWD_REGS_NEEDED);
+  if ((rc = check_regs(kern, checked_regs, fe::FWD_REGS_NEEDED, "tree attention"))) return rc;
   const int64_t items = (int64_t)p.B * p.Hkv * p.MT;
   if constexpr (CLUSTER) {
     cudaLaunchConfig_t cfg;
@@ -283,7 +293,7 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   p.D4 = (int)g.D4;
   p.nctas = (int)g.ctas;
   p.sc = (float)((double)scale * 1.4426950408889634);
-  p.tree_vec = tree && drafts % 16 == 0 && reinterpret_cast<uintptr_t>(tree) % 16 == 0 && tree_batch_stride % 16 == 0;
+  p.tree_vec = mask_is_vectors(tree, tree_batch_stride, drafts);
   p.timeout_ns = (uint64_t)g_watchdog_ns;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int dp = padded_dim(D);
@@ -332,6 +342,8 @@ int launch_commit(const CUtensorMap& tk, const CUtensorMap& tkn, fe::CommitParam
   auto kern = fe::fe_commit_mass_kernel<BF16, DP>;
   int rc = set_smem(kern, C::SMEM);
   if (rc) return rc;
+  static std::atomic<int> checked_regs{0};
+  if ((rc = check_regs(kern, checked_regs, fe::COMMIT_REGS_NEEDED, "commit"))) return rc;
   // The accepted count is on the device; A is its most.
   for (int64_t row0 = 0; row0 == 0 || row0 < (int64_t)p.A * p.G; row0 += C::ROWS) {
     p.row0 = (int)row0;
@@ -432,6 +444,7 @@ int fe_commit_tokens(const fe_cache* cache, const fe_cache* out, const void* q, 
   p.sc = (float)((double)scale * 1.4426950408889634);
   p.decay_log2 = (double)recency_decay * 1.4426950408889634;
   p.q_vec = rows_are_vectors(q, q_strides, B, q_heads, drafts, D) ? 1 : 0;
+  p.tree_vec = mask_is_vectors(tree, tree_batch_stride, drafts);
   p.timeout_ns = (uint64_t)g_watchdog_ns;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int dp = padded_dim(D);

@@ -130,38 +130,11 @@ __device__ __forceinline__ void tree_softmax_tile(float (&x)[128], bool first, b
 
 // Bit j of the 128: draft t sees draft j.
 __device__ __forceinline__ void tree_bits(const TreeParams& p, int b, int t, uint32_t (&bits)[4]) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) bits[w] = 0u;
-  if (p.tree == nullptr) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int n = min(max(t + 1 - 32 * w, 0), 32);
-      bits[w] = n == 32 ? 0xffffffffu : ((1u << n) - 1u);
-    }
-    return;
-  }
   const uint8_t* row = p.tree + b * p.tree_sb + static_cast<int64_t>(t) * p.T;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const int n = min(max(p.T - 32 * w, 0), 32);
-    uint32_t v = 0u;
-    if (p.tree_vec) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (16 * u >= n) continue;
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row + 32 * w) + u);
-        // Four mask bytes to four bits: 1 where nonzero, gathered by a multiply.
-        v |= ((__vsetgtu4(x.x, 0u) * 0x01020408u) >> 24) << (16 * u);
-        v |= ((__vsetgtu4(x.y, 0u) * 0x01020408u) >> 24) << (16 * u + 4);
-        v |= ((__vsetgtu4(x.z, 0u) * 0x01020408u) >> 24) << (16 * u + 8);
-        v |= ((__vsetgtu4(x.w, 0u) * 0x01020408u) >> 24) << (16 * u + 12);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < n) v |= (__ldg(row + 32 * w + j) != 0 ? 1u : 0u) << j;
-    }
-    bits[w] = v;
+    const int n = min(max((p.tree == nullptr ? t + 1 : p.T) - 32 * w, 0), 32);
+    bits[w] = p.tree == nullptr ? low_bits(n) : mask_word(row + 32 * w, n, p.tree_vec);
   }
 }
 
@@ -562,8 +535,7 @@ __global__ void __launch_bounds__(384, 1)
             uint32_t sees[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              const int n = min(max(lim + 1 - 32 * w, 0), 32);
-              sees[w] = drafts ? bits[w] : (n == 32 ? 0xffffffffu : ((1u << n) - 1u));
+              sees[w] = drafts ? bits[w] : low_bits(min(max(lim + 1 - 32 * w, 0), 32));
             }
             const bool masked = drafts || lim < 127;
             if (DUAL && !masked)  // the long runs' loop, free of masking code
