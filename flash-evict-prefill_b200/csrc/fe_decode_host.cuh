@@ -523,7 +523,7 @@ int fe_evict_tokens(const fe_cache* cache, const fe_cache* out, int64_t budget, 
   const bool smem_keys = held(cl) <= fe::SHRINK_SMEM_KEYS;
   auto kern = smem_keys ? fe::fe_shrink_kernel<true> : fe::fe_shrink_kernel<false>;
   const int smem = smem_keys ? (int)(held(cl) * 4) : 0;
-  if (smem > 32768 && (rc = set_smem(kern, fe::SHRINK_SMEM_KEYS * 4))) return rc;
+  if (smem > 16384 && (rc = set_smem(kern, fe::SHRINK_SMEM_KEYS * 4))) return rc;
   if (rows * cl > 0x7fffffff) return fail(FE_STATUS_UNSUPPORTED, "too many rows");
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));

@@ -16,11 +16,11 @@
 // order-preserving integer keys stay in shared memory (in registers the walks
 // over them have to be unrolled, and fetching that code once took longer than
 // running it: 46 us instead of XX for eight rows of 128K).  The budget-th largest key is
-// found by narrowing the range of the keys 256-fold a pass (bins of a power of
+// found by narrowing the range of the keys 1024-fold a pass (bins of a power of
 // two from the row's smallest key, so keys that share their top bits spread over
 // the bins all the same), histograms summed over distributed shared memory,
-// ending as soon as a bin's end coincides with the budget (two passes for a row
-// one token over).  Holes and movers are numbered by ballots in slot order,
+// ending as soon as a bin's end coincides with the budget (one or two passes for
+// a row of a few thousand).  Holes and movers are numbered by ballots in slot order,
 // listed, and copied by all warps of the cluster, eight rows a warp in flight.
 // Few rows are bound by the chain of cluster barriers, large batches by the
 // moved bytes.
@@ -55,10 +55,12 @@ struct ShrinkParams {
 
 constexpr int SHRINK_THREADS = 1024;
 constexpr int SHRINK_WARPS = SHRINK_THREADS / 32;
+static_assert(SHRINK_WARPS == 32, "scans give a lane to every warp");
 constexpr int SHRINK_MAX_CLUSTER = 8;
 // Keys a CTA holds.  (Clusters of 16 fit fewer than one to a GPC and ran eight
 // rows of 128K one after another.)
 constexpr int SHRINK_SMEM_KEYS = 49152;
+constexpr int SHRINK_BINS = 1024;  // bins of a pass, one a thread
 constexpr int SHRINK_LIST = 1024;  // moves listed in shared memory (one CTA a row)
 
 // Copies rows src[u] to rows dst[u], u < count <= U, of a cache's K and V by one
@@ -93,8 +95,8 @@ __device__ __forceinline__ void shrink_move(const ShrinkParams& p, uint8_t* kb, 
 template <bool HELD>
 __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __grid_constant__ ShrinkParams p) {
   extern __shared__ uint32_t skeys[];
-  __shared__ uint32_t hist[2][257];  // the last bin counts the reserved tokens
-  __shared__ __align__(16) uint32_t sums[3][260];  // rank 0: the cluster's histogram of a pass
+  __shared__ uint32_t hist[2][SHRINK_BINS + 1];  // the last bin counts the reserved tokens
+  __shared__ __align__(16) uint32_t sums[3][SHRINK_BINS + 4];  // rank 0: the cluster's histogram of a pass
   __shared__ int2 warp_count[2][SHRINK_WARPS];  // ties; holes and movers of each warp
   __shared__ int2 cta_count[2];
   __shared__ int found[3];
@@ -166,9 +168,9 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
         }
       }
     }
-    if (tid < 257) {
-      hist[0][tid] = hist[1][tid] = 0u;
-      sums[0][tid] = sums[1][tid] = sums[2][tid] = 0u;
+    for (int i = tid; i <= SHRINK_BINS; i += SHRINK_THREADS) {
+      hist[0][i] = hist[1][i] = 0u;
+      sums[0][i] = sums[1][i] = sums[2][i] = 0u;
     }
     newest = __reduce_max_sync(0xffffffffu, newest);
     lo = __reduce_min_sync(0xffffffffu, lo);
@@ -224,14 +226,14 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   int width = 32 - __clz(hi - lo), need = p.budget, ties = 0;
   uint32_t threshold = lo;
 #pragma unroll 1
-  for (int pass = 0; pass < 4; ++pass) {  // 32 bits, 8 a pass
-    const int shift = max(width - 8, 0);
+  for (int pass = 0; pass < 4; ++pass) {  // 32 bits, 10 a pass
+    const int shift = max(width - 10, 0);
     uint32_t* hh = hist[pass & 1];
     walk([&](int, bool valid, uint32_t k) {
       const bool reserved = k == 0xFFFFFFFFu;
       const uint32_t d = k - threshold;
       const bool in = valid && (reserved ? pass == 0 : width == 32 || (d >> width) == 0u);
-      const uint32_t bin = reserved ? 256u : d >> shift;
+      const uint32_t bin = reserved ? SHRINK_BINS : d >> shift;
       // The first candidate's bin once for all lanes that share it (weights of
       // exactly zero can be most of a row), the others one by one.
       const uint32_t any = __ballot_sync(0xffffffffu, in);
@@ -246,50 +248,42 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
     // next is added to, the one after is zeroed, between two cluster barriers).
     if (size > 1) {
       __syncthreads();
-      if (tid < 257 && hh[tid] != 0u) atomicAdd(cluster.map_shared_rank(&sums[pass % 3][tid], 0), hh[tid]);
+      for (int i = tid; i <= SHRINK_BINS; i += SHRINK_THREADS)
+        if (hh[i] != 0u) atomicAdd(cluster.map_shared_rank(&sums[pass % 3][i], 0), hh[i]);
     }
     sync();
-    if (tid >= 32 && tid < 32 + 257) {
-      hist[(pass + 1) & 1][tid - 32] = 0u;
-      sums[(pass + 2) % 3][tid - 32] = 0u;
+    const uint32_t* from = size > 1 ? cluster.map_shared_rank(&sums[pass % 3][0], 0) : hh;
+    const uint32_t cnt = from[tid], reserved = from[SHRINK_BINS];  // (only the first pass counts reserved tokens)
+    for (int i = tid; i <= SHRINK_BINS; i += SHRINK_THREADS) {
+      hist[(pass + 1) & 1][i] = 0u;
+      sums[(pass + 2) % 3][i] = 0u;
     }
-    if (warp == 0) {
-      uint32_t cnt[8];
-      uint32_t mine = 0;
-      const uint32_t* from = size > 1 ? cluster.map_shared_rank(&sums[pass % 3][0], 0) : hh;
-      const uint32_t reserved = from[256];  // above every bin (only the first pass counts them)
+    // The bin in which the count from above reaches `need`: a suffix sum.
+    uint32_t above = cnt;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        cnt[u] = from[lane * 8 + u];
-        mine += cnt[u];
-      }
-      uint32_t above = mine;  // inclusive suffix sum over the lanes
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_down_sync(0xffffffffu, above, o);
-        if (lane + o < 32) above += x;
-      }
-      uint32_t upper = reserved + above - mine;  // keys above this lane's bins
-      if (reserved >= static_cast<uint32_t>(need) && lane == 0) {
-        found[0] = 256;
-        found[1] = 0;
-        found[2] = static_cast<int>(reserved);
-      }
-#pragma unroll
-      for (int u = 7; u >= 0; --u) {
-        if (upper < static_cast<uint32_t>(need) && upper + cnt[u] >= static_cast<uint32_t>(need)) {
-          found[0] = lane * 8 + u;
-          found[1] = static_cast<int>(upper);
-          found[2] = static_cast<int>(cnt[u]);
-        }
-        upper += cnt[u];
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_down_sync(0xffffffffu, above, o);
+      if (lane + o < 32) above += x;
+    }
+    if (lane == 0) s_lo[warp] = above;
+    __syncthreads();
+    const uint32_t higher = __reduce_add_sync(0xffffffffu, lane > warp ? s_lo[lane] : 0u);
+    const uint32_t upper = reserved + higher + above - cnt;  // keys above this bin
+    if (upper < static_cast<uint32_t>(need) && upper + cnt >= static_cast<uint32_t>(need)) {
+      found[0] = tid;
+      found[1] = static_cast<int>(upper);
+      found[2] = static_cast<int>(cnt);
+    }
+    if (tid == 0 && reserved >= static_cast<uint32_t>(need)) {
+      found[0] = SHRINK_BINS;
+      found[1] = 0;
+      found[2] = static_cast<int>(reserved);
     }
     __syncthreads();
     const int bin = found[0];
     need -= found[1];
     ties = found[2];
-    if (bin == 256) {
+    if (bin == SHRINK_BINS) {
       threshold = 0xFFFFFFFFu;
       break;
     }
@@ -307,7 +301,6 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   auto scan = [&](int which, int2 mine, int2* total) -> int2 {
     if (lane == 0) warp_count[which][warp] = mine;
     __syncthreads();
-    static_assert(SHRINK_WARPS == 32, "a lane per warp");
     const int2 v = warp_count[which][lane];
     int2 before = make_int2(__reduce_add_sync(0xffffffffu, lane < warp ? v.x : 0),
                             __reduce_add_sync(0xffffffffu, lane < warp ? v.y : 0));
@@ -379,25 +372,39 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   const int b = row / p.Hkv, h = row - b * p.Hkv;
   uint8_t* kb = p.k + b * p.k_sb + h * p.k_sh;
   uint8_t* vb = p.v + b * p.v_sb + h * p.v_sh;
-  // Eight consecutive moves a warp: lane u < 8 knows the u-th.
+  // Eight consecutive moves a warp, lane u < 8 knowing the u-th; the next ones
+  // are looked up, and the bookkeeping read, while the rows are on their way.
   constexpr int U = 8;
-  for (int i0 = (rank * SHRINK_WARPS + warp) * U; i0 < moves; i0 += size * SHRINK_WARPS * U) {
+  const int step = size * SHRINK_WARPS * U;
+  int i0 = (rank * SHRINK_WARPS + warp) * U;
+  auto look = [&](int i) -> int2 {
+    if (lane >= U || i + lane >= moves) return make_int2(0, 0);
+    return local ? slist[i + lane] : make_int2(__ldcg(holes + i + lane), __ldcg(movers + i + lane));
+  };
+  int2 mine = look(i0);  // {hole, mover}
+  for (; i0 < moves; i0 += step) {
     const int count = min(U, moves - i0);
-    int my_dst = 0, my_src = 0;
+    const int2 next = look(i0 + step);
+    float m = 0.f, z = 0.f;
+    int at = 0;
     if (lane < count) {
-      my_dst = local ? slist[i0 + lane].x : __ldcg(holes + i0 + lane);
-      my_src = local ? slist[i0 + lane].y : __ldcg(movers + i0 + lane);
-      p.mass_out[base + my_dst] = mass[my_src];
-      p.pos_out[base + my_dst] = pos[my_src];
-      if (p.norms_in != nullptr) p.norms_out[base + my_dst] = p.norms_in[base + my_src];
+      m = mass[mine.y];
+      at = pos[mine.y];
+      if (p.norms_in != nullptr) z = p.norms_in[base + mine.y];
     }
     int src[U], dst[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      src[u] = __shfl_sync(0xffffffffu, my_src, u);
-      dst[u] = __shfl_sync(0xffffffffu, my_dst, u);
+      dst[u] = __shfl_sync(0xffffffffu, mine.x, u);
+      src[u] = __shfl_sync(0xffffffffu, mine.y, u);
     }
     shrink_move<U>(p, kb, vb, src, dst, count, lane);
+    if (lane < count) {
+      p.mass_out[base + mine.x] = m;
+      p.pos_out[base + mine.x] = at;
+      if (p.norms_in != nullptr) p.norms_out[base + mine.x] = z;
+    }
+    mine = next;
   }
 }
 
