@@ -15,15 +15,16 @@
 // One cluster of CTAs per row, every warp a contiguous stretch of slots whose
 // order-preserving integer keys stay in shared memory (in registers the walks
 // over them have to be unrolled, and fetching that code once took longer than
-// running it: 46 us instead of XX for eight rows of 128K).  The budget-th largest key is
+// running it: 46 us instead of 40 for eight rows of 128K, all else alike).  The budget-th largest key is
 // found by narrowing the range of the keys 1024-fold a pass (bins of a power of
 // two from the row's smallest key, so keys that share their top bits spread over
 // the bins all the same), histograms summed over distributed shared memory,
 // ending as soon as a bin's end coincides with the budget (one or two passes for
 // a row of a few thousand).  Holes and movers are numbered by ballots in slot order,
 // listed, and copied by all warps of the cluster, eight rows a warp in flight.
-// Few rows are bound by the chain of cluster barriers, large batches by the
-// moved bytes.
+// Where a CTA might have much to copy, a second launch splits all rows' moves
+// evenly instead (rows need very different numbers of them).  Few rows are bound
+// by the chain of cluster barriers, large batches by the moved bytes.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -48,8 +49,9 @@ struct ShrinkParams {
   int32_t* len_out;
   int32_t* holes;   // workspace [rows][list]
   int32_t* movers;  // workspace [rows][list]
+  int32_t* counts;  // workspace [rows]: moves of each row, or null: moved by this launch
   int64_t list;
-  int Hkv, capacity, budget, recent, row_bytes;
+  int rows, Hkv, capacity, budget, recent, row_bytes;
   int copy;  // the outputs are other buffers than the inputs
 };
 
@@ -90,6 +92,44 @@ __device__ __forceinline__ void shrink_move(const ShrinkParams& p, uint8_t* kb, 
       }
 }
 
+// Moves [i0, end) of a row, eight consecutive ones a warp at a time (`step`
+// apart), lane u < 8 knowing the u-th; the next ones are looked up, and the
+// bookkeeping read, while the rows are on their way.
+template <typename Look>
+__device__ __forceinline__ void shrink_moves(const ShrinkParams& p, int row, int i0, int end, int step, int lane, Look look) {
+  constexpr int U = 8;
+  const int b = row / p.Hkv, h = row - b * p.Hkv;
+  const int64_t base = static_cast<int64_t>(row) * p.capacity;
+  uint8_t* kb = p.k + b * p.k_sb + h * p.k_sh;
+  uint8_t* vb = p.v + b * p.v_sb + h * p.v_sh;
+  auto mine_of = [&](int i) { return lane < U && i + lane < end ? look(i + lane) : make_int2(0, 0); };
+  int2 mine = mine_of(i0);  // {hole, mover}
+  for (; i0 < end; i0 += step) {
+    const int count = min(U, end - i0);
+    const int2 next = mine_of(i0 + step);
+    float m = 0.f, z = 0.f;
+    int at = 0;
+    if (lane < count) {
+      m = p.mass_in[base + mine.y];
+      at = p.pos_in[base + mine.y];
+      if (p.norms_in != nullptr) z = p.norms_in[base + mine.y];
+    }
+    int src[U], dst[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      dst[u] = __shfl_sync(0xffffffffu, mine.x, u);
+      src[u] = __shfl_sync(0xffffffffu, mine.y, u);
+    }
+    shrink_move<U>(p, kb, vb, src, dst, count, lane);
+    if (lane < count) {
+      p.mass_out[base + mine.x] = m;
+      p.pos_out[base + mine.x] = at;
+      if (p.norms_in != nullptr) p.norms_out[base + mine.x] = z;
+    }
+    mine = next;
+  }
+}
+
 // HELD: the keys of a CTA's slots fit its shared memory; otherwise (longer rows)
 // they are made again from the weights on every walk.
 template <bool HELD>
@@ -107,6 +147,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   const int rank = static_cast<int>(cluster.block_rank()), size = static_cast<int>(cluster.num_blocks());
   const int row = static_cast<int>(blockIdx.x) / size;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
   const int n = cache_length(p.len_in, row, p.capacity);
   const int64_t base = static_cast<int64_t>(row) * p.capacity;
   const float* mass = p.mass_in + base;
@@ -125,7 +166,10 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
       }
     }
     sync();  // every CTA has read the length
-    if (rank == 0 && tid == 0) p.len_out[row] = n;
+    if (rank == 0 && tid == 0) {
+      p.len_out[row] = n;
+      if (p.counts != nullptr) p.counts[row] = 0;
+    }
     return;
   }
 
@@ -349,7 +393,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   int hole = start.x, mover = start.y;
   const int moves = total.x;  // as many holes as movers
   // One CTA with few moves lists them in shared memory.
-  const bool local = size == 1 && moves <= SHRINK_LIST;
+  const bool local = size == 1 && moves <= SHRINK_LIST && p.counts == nullptr;
   int32_t* holes = p.holes + static_cast<int64_t>(row) * p.list;
   int32_t* movers = p.movers + static_cast<int64_t>(row) * p.list;
   sweep([&](int i, bool valid, bool keep) {
@@ -369,42 +413,63 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   if (!local) __threadfence();
   sync();  // the lists are complete, and nobody reads a neighbour's shared memory any more
   if (rank == 0 && tid == 0) p.len_out[row] = p.budget;
-  const int b = row / p.Hkv, h = row - b * p.Hkv;
-  uint8_t* kb = p.k + b * p.k_sb + h * p.k_sh;
-  uint8_t* vb = p.v + b * p.v_sb + h * p.v_sh;
-  // Eight consecutive moves a warp, lane u < 8 knowing the u-th; the next ones
-  // are looked up, and the bookkeeping read, while the rows are on their way.
-  constexpr int U = 8;
-  const int step = size * SHRINK_WARPS * U;
-  int i0 = (rank * SHRINK_WARPS + warp) * U;
-  auto look = [&](int i) -> int2 {
-    if (lane >= U || i + lane >= moves) return make_int2(0, 0);
-    return local ? slist[i + lane] : make_int2(__ldcg(holes + i + lane), __ldcg(movers + i + lane));
-  };
-  int2 mine = look(i0);  // {hole, mover}
-  for (; i0 < moves; i0 += step) {
-    const int count = min(U, moves - i0);
-    const int2 next = look(i0 + step);
-    float m = 0.f, z = 0.f;
-    int at = 0;
-    if (lane < count) {
-      m = mass[mine.y];
-      at = pos[mine.y];
-      if (p.norms_in != nullptr) z = p.norms_in[base + mine.y];
-    }
-    int src[U], dst[U];
+  if (p.counts != nullptr) {
+    if (rank == 0 && tid == 0) p.counts[row] = moves;
+    return;
+  }
+  shrink_moves(p, row, (rank * SHRINK_WARPS + warp) * 8, moves, size * SHRINK_WARPS * 8, lane, [&](int i) {
+    return local ? slist[i] : make_int2(__ldcg(holes + i), __ldcg(movers + i));
+  });
+}
+
+constexpr int MOVE_THREADS = 512;
+
+// The rows' moves laid end to end, an equal run for every CTA.
+__global__ void __launch_bounds__(MOVE_THREADS, 1) fe_shrink_move_kernel(const __grid_constant__ ShrinkParams p) {
+  __shared__ int sums[MOVE_THREADS / 32];
+  __shared__ int found[2];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per_thread = (p.rows + MOVE_THREADS - 1) / MOVE_THREADS;
+  const int first = min(p.rows, static_cast<int>(threadIdx.x) * per_thread), last = min(p.rows, first + per_thread);
+  int mine = 0;
+  for (int i = first; i < last; ++i) mine += __ldcg(p.counts + i);
+  int incl = mine;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      dst[u] = __shfl_sync(0xffffffffu, mine.x, u);
-      src[u] = __shfl_sync(0xffffffffu, mine.y, u);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += n;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  int start = incl - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < MOVE_THREADS / 32; ++w) {
+    start += w < warp ? sums[w] : 0;
+    total += sums[w];
+  }
+  // Runs of whole groups of eight, so that a group of a row is not shared.
+  const int per = ((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x) + 7) & ~7;
+  const int lo = min(total, static_cast<int>(blockIdx.x) * per), hi = min(total, lo + per);
+  for (int i = first; i < last; ++i) {
+    const int n = __ldcg(p.counts + i);
+    if (lo < hi && start <= lo && lo < start + n) {
+      found[0] = i;
+      found[1] = start;
     }
-    shrink_move<U>(p, kb, vb, src, dst, count, lane);
-    if (lane < count) {
-      p.mass_out[base + mine.x] = m;
-      p.pos_out[base + mine.x] = at;
-      if (p.norms_in != nullptr) p.norms_out[base + mine.x] = z;
-    }
-    mine = next;
+    start += n;
+  }
+  __syncthreads();
+  if (lo >= hi) return;
+  int row = found[0], begin = found[1];  // first move of `row` in the whole
+  while (begin < hi) {
+    const int n = __ldcg(p.counts + row);
+    const int32_t* holes = p.holes + static_cast<int64_t>(row) * p.list;
+    const int32_t* movers = p.movers + static_cast<int64_t>(row) * p.list;
+    shrink_moves(p, row, max(lo - begin, 0) + warp * 8, min(hi - begin, n), MOVE_THREADS / 32 * 8, lane,
+                 [&](int i) { return make_int2(__ldcg(holes + i), __ldcg(movers + i)); });
+    begin += n;
+    ++row;
   }
 }
 

@@ -18,7 +18,7 @@
 // joins them in a fixed order (no atomics, bitwise reproducible).  Few short
 // rows (a decode step over compacted caches) are latency instead: there a
 // cluster of eight CTAs has a row and joins through distributed shared memory,
-// in one launch (CLUSTER; 12.4 -> XX us for 4 rows of 2048).
+// in one launch (CLUSTER; 12.4 -> 10.7 us for 4 rows of 2048).
 //
 // Roles (384 threads): warps 0-3 and 4-7 are two softmax warpgroups, warp 8
 // issues TMA, warp 9 tcgen05.mma.  Up to 128 rows (SPLIT) both warpgroups

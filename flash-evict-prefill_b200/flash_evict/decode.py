@@ -124,7 +124,7 @@ def _readable(t):
     """(tensor, its stride array): t if the kernels can read it in place, else a copy that they can."""
     st = t.stride()
     if st[3] != 1 or (st[0] | st[1] | st[2]) & 7 or t.data_ptr() & 15 or 0 in st:
-        t = _tma_view(t)
+        t = _tma_view(t.contiguous() if 0 in st else t)  # expanded dimensions are laid out
         st = t.stride()
     return t, _stride_array(st)
 

@@ -69,8 +69,8 @@ def test_c_abi_refusals_without_a_gpu():
     bad = (512, 256, 9, 1)
     assert evict(c_cache(k_strides=bad), c_cache(k_strides=bad)) == _lib.STATUS_UNSUPPORTED
     assert lib.fe_evict_workspace_bytes(ctypes.byref(c_cache()), 0) == -1
-    assert lib.fe_evict_workspace_bytes(ctypes.byref(c_cache()), 10) == 2 * 10 * 8
-    assert lib.fe_evict_workspace_bytes(ctypes.byref(c_cache()), 100) == 2 * 8
+    assert lib.fe_evict_workspace_bytes(ctypes.byref(c_cache()), 10) == 2 * (10 * 8 + 4)
+    assert lib.fe_evict_workspace_bytes(ctypes.byref(c_cache()), 100) == 2 * 12
 
 
 def test_cache_refuses_tensors_it_cannot_hold():

@@ -180,6 +180,16 @@ def test_layouts_and_streams():
     assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
 
 
+def test_expanded_inputs():
+    # one K/V head, one query and one mask for all: dimensions of stride 0
+    q, kn, vn, cache, gen = make(16, 2, 8, 4, 64, 300, 5, torch.float16, 200)
+    tree = random_tree(gen, 1, 5).cuda()
+    q, kn, vn = q[:, :1].expand_as(q), kn[:, :1].expand_as(kn), vn[:1].expand_as(vn)
+    got = check_attention(q, kn, vn, cache, tree=tree.expand(2, 5, 5))
+    ref = tree_attention(q.contiguous(), kn.contiguous(), vn.contiguous(), cache, tree=tree[0])
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
 def test_attention_in_a_graph_follows_the_lengths():
     q, kn, vn, cache, gen = make(15, 1, 8, 2, 128, 800, 1, torch.bfloat16, 300, junk=0.5)
     tree_attention(q, kn, vn, cache)

@@ -237,6 +237,17 @@ def test_evict_many_rows():
     check_evict(cache, 256, 20)
 
 
+def test_evict_many_rows_with_much_to_move():
+    # enough rows and bytes that the moves are a launch of their own
+    gen = torch.Generator().manual_seed(7)
+    lengths = torch.randint(0, 2301, (5, 8), generator=gen)
+    lengths[0, 0], lengths[4, 7], lengths[2, 3] = 0, 2300, 1101
+    cache, _ = cache_for_eviction(37, 5, 8, 128, 2300, lengths.tolist(), dtype=torch.float16)
+    check_evict(clone(cache), 1100, 64)
+    cache, _ = cache_for_eviction(38, 5, 8, 100, 2900, 2900, norms=False)
+    check_evict(cache, 1449, 0)
+
+
 def test_evict_ties_zeros_infinities_and_nan():
     cache, gen = cache_for_eviction(34, 1, 4, 32, 3000, 3000)
     m = cache.mass
