@@ -66,9 +66,9 @@ class KVCache:
             init(self, name, t)
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         b, h, c, d = k.shape
-        init(self, "_sync", None if mass is None else torch.zeros(1, dtype=torch.int32, device=k.device))
+        init(self, "_sync", None)  # made by the first commit in place
         init(self, "_c", _lib.Cache(k.data_ptr(), v.data_ptr(), k.stride(), v.stride(), ptr(mass), ptr(norms), ptr(positions),
-                                    lengths.data_ptr(), ptr(self._sync), b, h, c, d, _DTYPES[k.dtype]))
+                                    lengths.data_ptr(), None, b, h, c, d, _DTYPES[k.dtype]))
         init(self, "_ref", ctypes.byref(self._c))
         init(self, "_sizes", {})  # workspace bytes by the calls' shapes
         _lib.check(_lib.load().fe_cache_prepare(self._ref))
@@ -78,6 +78,11 @@ class KVCache:
 
     def __setattr__(self, name, value):
         raise AttributeError("a KVCache's tensors cannot be replaced; update them in place")
+
+    def _make_sync(self):
+        # The word that counts a commit's CTAs: zero before and after.
+        object.__setattr__(self, "_sync", torch.zeros(1, dtype=torch.int32, device=self.device))
+        self._c.sync = self._sync.data_ptr()
 
     @classmethod
     def allocate(cls, batch, kv_heads, capacity, channels, dtype=torch.bfloat16, device="cuda", *, value_weighted=True):
@@ -259,6 +264,8 @@ def commit_tokens(cache, q, k_new, v_new, lse, accepted, positions, *, tree=None
     recency_decay = float(recency_decay)
     if not math.isfinite(recency_decay) or recency_decay < 0:
         raise ValueError("recency_decay must be finite and nonnegative")
+    if out is cache and cache._sync is None:
+        cache._make_sync()
     lib = _lib.load()
     a = accepted.shape[1]
     size, workspace, pointer = _workspace(cache, (hq, t, a, out is cache), lib.fe_commit_workspace_bytes, cache._ref, out._ref, hq, t, a)
