@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
 
+  pdl_launch_dependents();
   if (threadIdx.x == C::PRODUCER * 32) {
     tma_prefetch_desc(&tk);
     tma_prefetch_desc(&tkn);
@@ -300,6 +301,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
     tmem_relinquish();
   }
   tc_fence_before();
+  pdl_wait();  // nothing above reads or writes memory
   DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, 1, COMMIT_EXTRA, blockIdx.x, p.nctas,
                                                scratch);
   tc_fence_after();

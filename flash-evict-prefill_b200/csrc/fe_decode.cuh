@@ -188,8 +188,11 @@ __device__ __forceinline__ float elem_to_float(uint16_t x) {
   else return __half2float(__ushort_as_half(x));
 }
 
-// Programmatic dependent launch: let the next kernel of the stream start
-// (its prologue only), and wait for the previous one's writes.
+// Programmatic dependent launch: let the next kernel of the stream start (its
+// prologue only), and wait until the previous ones are done and their writes
+// are seen.  Every decode kernel is launched so and touches no memory before the
+// wait, so whatever ran before it, decode kernel or not, it only overlaps that
+// one's tail with its own start (barriers, TMEM, descriptors).
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

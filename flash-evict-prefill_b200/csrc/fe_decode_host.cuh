@@ -133,18 +133,26 @@ int check_regs(Kern kern, std::atomic<int>& checked, int needed, const char* wha
   return FE_STATUS_OK;
 }
 
+// Launches with programmatic stream serialization (the kernel waits for what is
+// before it in the stream by itself), in clusters of `cluster` CTAs.
 template <typename Kern, typename... Args>
-int launch_dependent(Kern kern, dim3 grid, dim3 block, cudaStream_t stream, const char* what, Args... args) {
+int launch_dependent(Kern kern, dim3 grid, dim3 block, int smem, int cluster, cudaStream_t stream, const char* what,
+                     Args... args) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) return cuda_fail(e, what);
   return FE_STATUS_OK;
@@ -160,27 +168,9 @@ int launch_tree(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
   static std::atomic<int> checked_regs{0};
   if ((rc = check_regs(kern, checked_regs, fe::FWD_REGS_NEEDED, "tree attention"))) return rc;
   const int64_t items = (int64_t)p.B * p.Hkv * p.MT;
-  if constexpr (CLUSTER) {
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3((unsigned)(items * fe::TREE_CLUSTER));
-    cfg.blockDim = dim3(C::THREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = fe::TREE_CLUSTER;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, tkn, tvn, p);
-    if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
-    return FE_STATUS_OK;
-  }
-  kern<<<dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, stream>>>(tq, tk, tv, tkn, tvn, p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
+  rc = launch_dependent(kern, dim3((unsigned)(CLUSTER ? items * fe::TREE_CLUSTER : p.nctas)), dim3(C::THREADS), C::SMEM,
+                        CLUSTER ? fe::TREE_CLUSTER : 1, stream, "tree attention launch", tq, tk, tv, tkn, tvn, p);
+  if (rc || CLUSTER) return rc;
   // Warps that share a row's partials: one per two partials (about ctas / items
   // of them), as long as the blocks are all resident at once (two an SM).
   const int64_t groups = (p.D4 / 4 + fe::TREE_JOIN_QUADS - 1) / fe::TREE_JOIN_QUADS, pairs = p.R * groups;
@@ -191,7 +181,7 @@ int launch_tree(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
   int splits = 1;
   while (splits < fe::TREE_JOIN_WARPS && splits * 2 * items < p.nctas && blocks(2 * splits) * items <= 2 * p.nctas) splits *= 2;
   return launch_dependent(fe::fe_tree_join_kernel<BF16>, dim3((unsigned)items, (unsigned)blocks(splits)),
-                          dim3(fe::TREE_JOIN_THREADS), stream, "tree join launch", p, C::QTILES * p.tile_rows, splits);
+                          dim3(fe::TREE_JOIN_THREADS), 0, 1, stream, "tree join launch", p, C::QTILES * p.tile_rows, splits);
 }
 
 template <bool BF16>
@@ -348,9 +338,8 @@ int launch_commit(const CUtensorMap& tk, const CUtensorMap& tkn, fe::CommitParam
   for (int64_t row0 = 0; row0 == 0 || row0 < (int64_t)p.A * p.G; row0 += C::ROWS) {
     p.row0 = (int)row0;
     p.last = row0 + C::ROWS >= (int64_t)p.A * p.G;
-    kern<<<dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, stream>>>(tk, tkn, p);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_fail(e, "commit launch");
+    rc = launch_dependent(kern, dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, 1, stream, "commit launch", tk, tkn, p);
+    if (rc) return rc;
   }
   return FE_STATUS_OK;
 }
@@ -532,24 +521,10 @@ int fe_evict_tokens(const fe_cache* cache, const fe_cache* out, int64_t budget, 
   const int smem = smem_keys ? (int)(held(cl) * 4) : 0;
   if (smem > 16384 && (rc = set_smem(kern, fe::SHRINK_SMEM_KEYS * 4))) return rc;
   if (rows * cl > 0x7fffffff) return fail(FE_STATUS_UNSUPPORTED, "too many rows");
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)(rows * cl));
-  cfg.blockDim = dim3(fe::SHRINK_THREADS);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cl;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-  if (e != cudaSuccess) return cuda_fail(e, "cache eviction launch");
-  if (!two) return FE_STATUS_OK;
-  return launch_dependent(fe::fe_shrink_move_kernel, dim3(sm_count(dev)), dim3(fe::MOVE_THREADS),
-                          reinterpret_cast<cudaStream_t>(stream), "cache move launch", p);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  rc = launch_dependent(kern, dim3((unsigned)(rows * cl)), dim3(fe::SHRINK_THREADS), smem, cl, s, "cache eviction launch", p);
+  if (rc || !two) return rc;
+  return launch_dependent(fe::fe_shrink_move_kernel, dim3(sm_count(dev)), dim3(fe::MOVE_THREADS), 0, 1, s, "cache move launch", p);
 }
 
 }  // extern "C"

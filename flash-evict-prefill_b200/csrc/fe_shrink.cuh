@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   const int row = static_cast<int>(blockIdx.x) / size;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
+  pdl_wait();
   const int n = cache_length(p.len_in, row, p.capacity);
   const int64_t base = static_cast<int64_t>(row) * p.capacity;
   const float* mass = p.mass_in + base;
@@ -428,6 +429,7 @@ constexpr int MOVE_THREADS = 512;
 __global__ void __launch_bounds__(MOVE_THREADS, 1) fe_shrink_move_kernel(const __grid_constant__ ShrinkParams p) {
   __shared__ int sums[MOVE_THREADS / 32];
   __shared__ int found[2];
+  pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per_thread = (p.rows + MOVE_THREADS - 1) / MOVE_THREADS;

@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(384, 1)
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = threadIdx.x & 31;
 
-  if constexpr (!CLUSTER) pdl_launch_dependents();
+  pdl_launch_dependents();
   if (threadIdx.x == 256) {
     tma_prefetch_desc(&tq);
     tma_prefetch_desc(&tk);
@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(384, 1)
     tmem_relinquish();
   }
   tc_fence_before();
+  pdl_wait();  // nothing above reads or writes memory
   DecWalk walk;
   if constexpr (CLUSTER) {
     // A CTA of the cluster has an eighth of one item's tiles.
@@ -695,6 +696,7 @@ __global__ void __launch_bounds__(TREE_JOIN_THREADS)
   __shared__ float4 s_acc[TREE_JOIN_WARPS][Q][32];
   __shared__ float2 s_ml[TREE_JOIN_WARPS][32];
   __shared__ int scratch[TREE_JOIN_WARPS], s_start;
+  pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int split = warp % splits;
   const int quads = p.D4 / 4, groups = (quads + Q - 1) / Q;
