@@ -517,8 +517,9 @@ int fe_evict_tokens(const fe_cache* cache, const fe_cache* out, int64_t budget, 
   while (cl < fe::SHRINK_MAX_CLUSTER && held(cl) > fe::SHRINK_SMEM_KEYS) cl *= 2;
   while (cl < fe::SHRINK_MAX_CLUSTER && rows * cl * (two ? 2 : 1) <= sm_count(dev) && cap / (2 * cl) >= 2048) cl *= 2;
   const bool smem_keys = held(cl) <= fe::SHRINK_SMEM_KEYS;
+  p.hold_positions = smem_keys && recent > 0 && 2 * held(cl) <= fe::SHRINK_SMEM_KEYS;
   auto kern = smem_keys ? fe::fe_shrink_kernel<true> : fe::fe_shrink_kernel<false>;
-  const int smem = smem_keys ? (int)(held(cl) * 4) : 0;
+  const int smem = smem_keys ? (int)(held(cl) * (p.hold_positions ? 8 : 4)) : 0;
   if (smem > 16384 && (rc = set_smem(kern, fe::SHRINK_SMEM_KEYS * 4))) return rc;
   if (rows * cl > 0x7fffffff) return fail(FE_STATUS_UNSUPPORTED, "too many rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -53,6 +53,7 @@ struct ShrinkParams {
   int64_t list;
   int rows, Hkv, capacity, budget, recent, row_bytes;
   int copy;  // the outputs are other buffers than the inputs
+  int hold_positions;  // shared memory holds the positions, too
 };
 
 constexpr int SHRINK_THREADS = 1024;
@@ -136,7 +137,7 @@ template <bool HELD>
 __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __grid_constant__ ShrinkParams p) {
   extern __shared__ uint32_t skeys[];
   __shared__ uint32_t hist[2][SHRINK_BINS + 1];  // the last bin counts the reserved tokens
-  __shared__ __align__(16) uint32_t sums[3][SHRINK_BINS + 4];  // rank 0: the cluster's histogram of a pass
+  __shared__ __align__(16) uint32_t sums[3][SHRINK_BINS + 4];  // the cluster's histogram of a pass, each CTA some bins
   __shared__ int2 warp_count[2][SHRINK_WARPS];  // ties; holes and movers of each warp
   __shared__ int2 cta_count[2];
   __shared__ int found[3];
@@ -180,6 +181,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   const int steps = (w1 - w0 + 31) >> 5;
 
   uint32_t* wkeys = skeys + warp * wlen;
+  int* wpos = reinterpret_cast<int*>(skeys + SHRINK_WARPS * wlen) + warp * wlen;  // p.hold_positions
   int first_reserved = 0;  // positions from here on are reserved (recent > 0)
   uint32_t lo = 0xFFFFFFFFu, hi = 0u;  // range of the row's weights
   auto mass_key = [&](float m) -> uint32_t { return min(order_key(m), 0xFFFFFFFEu); };  // NaN above +inf, below the reserved
@@ -204,7 +206,10 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
         lo = min(lo, k);
         hi = max(hi, k);
         newest = max(newest, at[u]);
-        if (HELD && i < w1) wkeys[(j0 + u) * 32 + lane] = k;
+        if (HELD && i < w1) {
+          wkeys[(j0 + u) * 32 + lane] = k;
+          if (p.hold_positions) wpos[(j0 + u) * 32 + lane] = at[u];
+        }
         if (p.copy && i < min(w1, p.budget)) {
           // The evicted ones are overwritten after a barrier.
           p.mass_out[base + i] = m[u];
@@ -243,7 +248,13 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
     }
     first_reserved =
         static_cast<int>(max(static_cast<int64_t>(newest) - p.recent + 1, static_cast<int64_t>(-0x80000000LL)));
-    if (HELD && p.recent > 0) {
+    if (HELD && p.recent > 0 && p.hold_positions) {
+#pragma unroll 4
+      for (int j = 0; j < steps; ++j) {
+        const int i = j * 32 + lane;
+        if (w0 + i < w1 && wpos[i] >= first_reserved) wkeys[i] = 0xFFFFFFFFu;
+      }
+    } else if (HELD && p.recent > 0) {
       for (int j0 = 0; j0 < steps; j0 += 8) {
         int at[8];
 #pragma unroll
@@ -267,6 +278,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   };
 
   // ---- the budget-th largest key
+  const int owner = tid * size / SHRINK_BINS;  // CTA that gathers this thread's bin
   // Candidates are the keys in [lo, lo + 2^width); bins of 2^shift of them.
   int width = 32 - __clz(hi - lo), need = p.budget, ties = 0;
   uint32_t threshold = lo;
@@ -289,16 +301,18 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
       if (lane == first) atomicAdd(&hh[bin], static_cast<uint32_t>(__popc(same)));
       else if (in && !((same >> lane) & 1u)) atomicAdd(&hh[bin], 1u);
     });
-    // The cluster's histogram gathers in rank 0 (three buffers: one is read, the
-    // next is added to, the one after is zeroed, between two cluster barriers).
+    // The cluster's histogram gathers in three buffers: one is read, the next is
+    // added to, the one after is zeroed, between two cluster barriers.
     if (size > 1) {
       __syncthreads();
-      for (int i = tid; i <= SHRINK_BINS; i += SHRINK_THREADS)
-        if (hh[i] != 0u) atomicAdd(cluster.map_shared_rank(&sums[pass % 3][i], 0), hh[i]);
+      // Every CTA gathers its share of the bins.
+      if (hh[tid] != 0u) atomicAdd(cluster.map_shared_rank(&sums[pass % 3][tid], owner), hh[tid]);
+      if (tid == 0 && hh[SHRINK_BINS] != 0u) atomicAdd(cluster.map_shared_rank(&sums[pass % 3][SHRINK_BINS], 0), hh[SHRINK_BINS]);
     }
     sync();
-    const uint32_t* from = size > 1 ? cluster.map_shared_rank(&sums[pass % 3][0], 0) : hh;
-    const uint32_t cnt = from[tid], reserved = from[SHRINK_BINS];  // (only the first pass counts reserved tokens)
+    const uint32_t cnt = size > 1 ? *cluster.map_shared_rank(&sums[pass % 3][tid], owner) : hh[tid];
+    const uint32_t reserved =  // (only the first pass counts reserved tokens)
+        size > 1 ? *cluster.map_shared_rank(&sums[pass % 3][SHRINK_BINS], 0) : hh[SHRINK_BINS];
     for (int i = tid; i <= SHRINK_BINS; i += SHRINK_THREADS) {
       hist[(pass + 1) & 1][i] = 0u;
       sums[(pass + 2) % 3][i] = 0u;
