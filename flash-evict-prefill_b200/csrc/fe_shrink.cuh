@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
         lo = min(lo, k);
         hi = max(hi, k);
         newest = max(newest, at[u]);
-        if (HELD && i < w1) {
-          wkeys[(j0 + u) * 32 + lane] = k;
+        if (HELD && j0 + u < steps) {
+          wkeys[(j0 + u) * 32 + lane] = i < w1 ? k : 0u;  // past the row's end: below every weight
           if (p.hold_positions) wpos[(j0 + u) * 32 + lane] = at[u];
         }
         if (p.copy && i < min(w1, p.budget)) {
@@ -266,41 +266,48 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
     }
     __syncwarp();
   }
-  // Calls f(slot, valid, key) for the warp's slots, 32 at a time in order.
+  // Calls f(slot, key) for the warp's slots, 32 at a time in order; the key is 0,
+  // below every weight's, past the row's end.
   auto walk = [&](auto f) {
-#pragma unroll 2
+#pragma unroll 4
     for (int j = 0; j < steps; ++j) {
       const int i = w0 + j * 32 + lane;
       uint32_t k = 0u;
-      if (i < w1) k = HELD ? wkeys[j * 32 + lane] : as_key(mass_key(mass[i]), p.recent > 0 ? pos[i] : 0);
-      f(i, i < w1, k);
+      if (HELD) k = wkeys[j * 32 + lane];
+      else if (i < w1) k = as_key(mass_key(mass[i]), p.recent > 0 ? pos[i] : 0);
+      f(i, k);
     }
   };
 
   // ---- the budget-th largest key
   const int owner = tid * size / SHRINK_BINS;  // CTA that gathers this thread's bin
-  // Candidates are the keys in [lo, lo + 2^width); bins of 2^shift of them.
-  int width = 32 - __clz(hi - lo), need = p.budget, ties = 0;
-  uint32_t threshold = lo;
+  // Candidates are the keys in [threshold, threshold + span]; bins of 2^shift of
+  // them.  (A reserved token's key is above any such range.)
+  uint32_t threshold = lo, span = hi - lo;
+  int need = p.budget, ties = 0;
 #pragma unroll 1
   for (int pass = 0; pass < 4; ++pass) {  // 32 bits, 10 a pass
-    const int shift = max(width - 10, 0);
+    const int shift = max(22 - __clz(span), 0);
     uint32_t* hh = hist[pass & 1];
-    walk([&](int, bool valid, uint32_t k) {
-      const bool reserved = k == 0xFFFFFFFFu;
+    int reserved_here = 0;
+    walk([&](int, uint32_t k) {
       const uint32_t d = k - threshold;
-      const bool in = valid && (reserved ? pass == 0 : width == 32 || (d >> width) == 0u);
-      const uint32_t bin = reserved ? SHRINK_BINS : d >> shift;
-      // The first candidate's bin once for all lanes that share it (weights of
-      // exactly zero can be most of a row), the others one by one.
-      const uint32_t any = __ballot_sync(0xffffffffu, in);
-      if (any == 0u) return;
-      const int first = __ffs(any) - 1;
-      const uint32_t first_bin = __shfl_sync(0xffffffffu, bin, first);  // by all lanes: not inside a condition
-      const uint32_t same = __ballot_sync(0xffffffffu, in && bin == first_bin);
-      if (lane == first) atomicAdd(&hh[bin], static_cast<uint32_t>(__popc(same)));
-      else if (in && !((same >> lane) & 1u)) atomicAdd(&hh[bin], 1u);
+      const bool in = d <= span;
+      // Lane 0's bin once for all lanes that share it (weights of exactly zero
+      // can be most of a row), the others one by one.
+      const uint32_t bin = in ? d >> shift : SHRINK_BINS;
+      const uint32_t first_bin = __shfl_sync(0xffffffffu, bin, 0);
+      const uint32_t same = __ballot_sync(0xffffffffu, bin == first_bin);
+      if (in) {
+        if (bin != first_bin) atomicAdd(&hh[bin], 1u);
+        else if (lane == 0) atomicAdd(&hh[bin], static_cast<uint32_t>(__popc(same)));
+      }
+      reserved_here += k == 0xFFFFFFFFu ? 1 : 0;
     });
+    if (pass == 0 && p.recent > 0) {
+      reserved_here = __reduce_add_sync(0xffffffffu, reserved_here);
+      if (lane == 0 && reserved_here > 0) atomicAdd(&hh[SHRINK_BINS], static_cast<uint32_t>(reserved_here));
+    }
     // The cluster's histogram gathers in three buffers: one is read, the next is
     // added to, the one after is zeroed, between two cluster barriers.
     if (size > 1) {
@@ -349,7 +356,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
     threshold += static_cast<uint32_t>(bin) << shift;
     // Done when all keys of this bin stay, or it holds one key.
     if (ties == need || shift == 0) break;
-    width = shift;
+    span = (1u << shift) - 1u;
     __syncthreads();
   }
   const int keep_ties = need;  // of `ties` keys equal to it, the first ones stay
@@ -381,29 +388,32 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   int2 total;
   if (split_ties) {
     int c = 0;
-    walk([&](int, bool valid, uint32_t k) { c += valid && k == threshold ? 1 : 0; });
+    walk([&](int, uint32_t k) { c += k == threshold ? 1 : 0; });
     c = __reduce_add_sync(0xffffffffu, c);
     tie_base = scan(0, make_int2(c, 0), &total).x;
   }
-  // Calls f(slot, valid, kept) in order.
+  // Calls f(slot, kept) in order.
   auto sweep = [&](auto f) {
     int seen = tie_base;
-    walk([&](int i, bool valid, uint32_t k) {
-      bool keep = valid && k >= threshold;
+    walk([&](int i, uint32_t k) {
+      bool keep = k >= threshold;
       if (split_ties) {
-        const bool tie = valid && k == threshold;
+        const bool tie = k == threshold;
         const uint32_t bal = __ballot_sync(0xffffffffu, tie);
         if (tie) keep = seen + __popc(bal & below) < keep_ties;
         seen += __popc(bal);
       }
-      f(i, valid, keep);
+      f(i, keep);
     });
   };
+  // Slots past the row's end are above the budget and not kept: neither.
   int nh = 0, nm = 0;
-  sweep([&](int i, bool valid, bool keep) {
-    nh += __popc(__ballot_sync(0xffffffffu, valid && !keep && i < p.budget));
-    nm += __popc(__ballot_sync(0xffffffffu, keep && i >= p.budget));
+  sweep([&](int i, bool keep) {
+    nh += !keep && i < p.budget ? 1 : 0;
+    nm += keep && i >= p.budget ? 1 : 0;
   });
+  nh = __reduce_add_sync(0xffffffffu, nh);
+  nm = __reduce_add_sync(0xffffffffu, nm);
   const int2 start = scan(1, make_int2(nh, nm), &total);
   int hole = start.x, mover = start.y;
   const int moves = total.x;  // as many holes as movers
@@ -411,8 +421,8 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 1) fe_shrink_kernel(const __gr
   const bool local = size == 1 && moves <= SHRINK_LIST && p.counts == nullptr;
   int32_t* holes = p.holes + static_cast<int64_t>(row) * p.list;
   int32_t* movers = p.movers + static_cast<int64_t>(row) * p.list;
-  sweep([&](int i, bool valid, bool keep) {
-    const bool is_hole = valid && !keep && i < p.budget, is_mover = keep && i >= p.budget;
+  sweep([&](int i, bool keep) {
+    const bool is_hole = !keep && i < p.budget, is_mover = keep && i >= p.budget;
     const uint32_t bh = __ballot_sync(0xffffffffu, is_hole), bm = __ballot_sync(0xffffffffu, is_mover);
     if (is_hole) {
       if (local) slist[hole + __popc(bh & below)].x = i;
