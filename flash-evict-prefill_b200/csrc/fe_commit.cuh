@@ -32,7 +32,9 @@
 namespace fe {
 
 constexpr int COMMIT_MAX_ACCEPTED = 128;
-constexpr int COMMIT_EXTRA = 2;  // key tiles that beginning a row costs
+// Key tiles that beginning a row costs (batch of 16: 35.5 us with none, 33.0 with
+// 2, 32.2 with 3; 5 drafts of 64 over 32k 18.8, 14.8, 16.5).
+constexpr int COMMIT_EXTRA = 2;
 
 struct CommitParams {
   const uint16_t* q;

@@ -83,7 +83,9 @@ struct TreeCfg {
 // Lowest running max: finite, so that a row which has seen no key yet rescales
 // by 2^-huge = 0 and never forms inf - inf.
 constexpr float TREE_M0 = -3.0e38f;
-constexpr int TREE_EXTRA = 2;  // key tiles that beginning and ending a row cost
+// Key tiles that beginning and ending a row cost (batch of 16: 61.6 us with none,
+// 58.2, 54.9, 53.8 and 53.3 with 1 to 4; 64 drafts over 32k 53.7, 51.2, 49.6, 50.4, 50.2).
+constexpr int TREE_EXTRA = 3;
 constexpr uint32_t TREE_QBUF = 8192;  // bytes between the halves of a query tile's 64-column group
 
 // One key tile of a row's softmax (S in x).  With `masked`, only columns with
