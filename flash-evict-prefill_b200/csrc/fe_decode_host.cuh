@@ -240,8 +240,8 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   if (!std::isfinite(scale)) return fail(FE_STATUS_INVALID, "scale must be finite");
   if (q_strides[3] != 1) return fail(FE_STATUS_UNSUPPORTED, "q: channel stride must be 1");
   if (tree_batch_stride < 0) return fail(FE_STATUS_INVALID, "tree_batch_stride must be nonnegative");
-  if (reinterpret_cast<uintptr_t>(out) % 8 || reinterpret_cast<uintptr_t>(workspace) % 256)
-    return fail(FE_STATUS_UNSUPPORTED, "out must be 8-byte and workspace 256-byte aligned");
+  if (reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(FE_STATUS_UNSUPPORTED, "out must be 16-byte and workspace 256-byte aligned");
   int dev = 0;
   if ((rc = enter(cache->k, stream, &dev))) return rc;
   const int64_t B = cache->batch, H = cache->kv_heads, D = cache->channels;

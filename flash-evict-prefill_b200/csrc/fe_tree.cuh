@@ -75,7 +75,7 @@ struct TreeCfg {
   static constexpr int NBAR = 4 + 4 * STAGES + 7;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int OFF_ML = OFF_MISC + 16 + 64 + DEC_SCRATCH_INTS * 4;  // float2[128]
-  static constexpr int SMEM = OFF_ML + (SPLIT ? 128 * 8 : 0) + 1024;
+  static constexpr int SMEM = OFF_ML + 128 * 8 + 1024;
   static_assert(SMEM <= 232448, "shared memory of a CTA");
   static constexpr int THREADS = 384;
 };
@@ -459,10 +459,10 @@ __global__ void __launch_bounds__(384, 1)
       const float sc = p.sc;
       const bool sc_pos = sc > 0.f;
       const float sce = sc_pos ? sc : 1.0f;
-      // CLUSTER: the partial stays in shared memory, in the place of the tiles
-      // (every load has landed and every product has read them by then).
+      // CLUSTER: the partial stays in shared memory, O in the place of the tiles
+      // (every load has landed and every product has read them by then; after an
+      // abort it may be overwritten, but not the NaN statistics in s_ml).
       float4* s_part = reinterpret_cast<float4*>(smem);
-      float2* s_part_stats = reinterpret_cast<float2*>(smem + C::OFF_BAR - 128 * 8);
       bool ok = true;
       uint32_t it0 = 0, nseg = 0, ns = 0;  // key tiles before, segments, S tiles of this group
       for (; walk.next(sg); ++nseg) {
@@ -581,7 +581,6 @@ __global__ void __launch_bounds__(384, 1)
         const int64_t slot = static_cast<int64_t>(sg.bh) * p.MT + sg.mt + blockIdx.x;
         const int64_t orow = static_cast<int64_t>(sg.bh) * p.M + row;
         float4* dst = CLUSTER ? s_part + pr : p.acc + slot * p.R * (p.D4 / 4) + pr;
-        float2* dst_stats = CLUSTER ? s_part_stats : p.stats + slot * p.R;
         uint16_t* out = p.out + orow * p.D;
         // Special rows are added in memory, so such a run's sum goes through it.
         const bool special_rows = has_drafts && (spec[0] | spec[1] | spec[2] | spec[3]) != 0u;
@@ -589,7 +588,7 @@ __global__ void __launch_bounds__(384, 1)
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         if (live && (!C::SPLIT || t == 0)) {
           if (whole) p.lse[orow] = l == 0.f ? -INFINITY : (m_used + log2f(l)) * 0.69314718055994531f;
-          else dst_stats[pr] = make_float2(m_used, l);
+          else if (!CLUSTER) p.stats[slot * p.R + pr] = make_float2(m_used, l);
         }
         if (warp_live) {
           constexpr int CB = C::SPLIT ? DP / 2 : DP;
@@ -639,11 +638,12 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
         tc_fence_before();
-        if constexpr (C::SPLIT) named_bar_sync(3, 256);  // both are done with both O tiles
+        if constexpr (C::SPLIT) named_bar_sync(3, 256);  // both are done with both O tiles and with s_ml
+        if (CLUSTER && t == 0) s_ml[r] = make_float2(m_used, l);
         it0 += ntile;
       }
       if constexpr (CLUSTER) {
-        if (nseg == 0 && t == 0) s_part_stats[r] = make_float2(TREE_M0, 0.f);
+        if (nseg == 0 && t == 0) s_ml[r] = make_float2(TREE_M0, 0.f);  // no tile of its own
         cluster_barrier();
         // Every CTA joins an eighth of the item's rows and channels.
         cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
@@ -657,7 +657,7 @@ __global__ void __launch_bounds__(384, 1)
           float4 v[TREE_CLUSTER][1];
 #pragma unroll
           for (int c = 0; c < TREE_CLUSTER; ++c) {
-            st[c] = *cluster.map_shared_rank(s_part_stats + rr, c);
+            st[c] = *cluster.map_shared_rank(s_ml + rr, c);
             v[c][0] = *cluster.map_shared_rank(s_part + quad * p.R + rr, c);
           }
           TreeMerge<1> sum;

@@ -6,6 +6,9 @@ sm_100a native library bound by `_lib`.  `gather_tokens`,
 `select_and_gather` and `evict_compact` (flash_evict.compact) add the KV
 compaction the reference's adapters perform after selection;
 `check_status` reports failures of kernels launched by earlier calls.
+`flash_evict.decode` decodes over the compacted cache (attention of drafted
+tokens, commit, eviction); `flash_evict.policies`, `flash_evict.baselines`,
+`flash_evict.distributed` and `flash_evict.streaming_adapter` hold the rest.
 """
 from .prefill import prefill, evict, select_tokens
 from .compact import gather_tokens, select_and_gather, evict_compact

@@ -119,12 +119,25 @@ def test_tree_attention_ragged_rows():
     check_attention(q, kn, vn, cache, tree=tree[1].cuda())
 
 
-def test_tree_attention_many_short_rows():
-    # far more rows than SMs: each run covers several rows
+@pytest.mark.parametrize("d", [64, 20, 81, 200])
+def test_tree_attention_many_short_rows(d):
+    # far more rows than SMs: each run covers several rows and writes most of them itself
     gen = torch.Generator().manual_seed(3)
-    lengths = torch.randint(0, 400, (60, 8), generator=gen).tolist()
-    q, kn, vn, cache, _ = make(8, 60, 16, 8, 64, 400, 2, torch.float16, lengths)
+    lengths = torch.randint(0, 400, (40, 8), generator=gen).tolist()
+    q, kn, vn, cache, _ = make(8, 40, 16, 8, d, 400, 2, torch.float16, lengths)
     check_attention(q, kn, vn, cache)
+
+
+@pytest.mark.parametrize("b,hq,hk,d,t", [(3, 16, 8, 128, 6), (3, 16, 8, 72, 5), (2, 30, 10, 256, 4), (1, 5, 1, 200, 3), (2, 24, 2, 64, 20)])
+def test_masked_drafts_in_every_kernel_shape(b, hq, hk, d, t):
+    # one row a run and several, one warpgroup and two, one query tile and two
+    for lengths in (0, 3, 260):
+        q, kn, vn, cache, gen = make(17 + lengths, b, hq, hk, d, 300, t, torch.bfloat16, lengths)
+        tree = random_tree(gen, 1, t)[0]
+        tree[:, t - 1] = False
+        kn[:, :, t - 1], vn[:, :, t - 1] = float("nan"), float("-inf")
+        vn[:, :, 1, 3] = float("inf")
+        check_attention(q, kn, vn, cache, tree=tree.cuda())
 
 
 def test_tree_attention_long_row_is_shared():
