@@ -273,6 +273,53 @@ def test_positions_at_the_ends_of_their_range():
     check_evict(clone(cache), 299, 299)
 
 
+def test_offsets_past_32_bits():
+    """A [B, C, H, D] cache of 2.5 G elements a tensor: head 0's last slots and head 8's first lie past 2^31 elements."""
+    cap, h, d, t = 1_100_000, 9, 256, 2
+    gen = torch.Generator().manual_seed(8)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    k, v = (torch.empty(1, cap, h, d, dtype=torch.bfloat16, device="cuda").normal_(generator=g).transpose(1, 2) for _ in range(2))
+    n = cap - 100
+    lengths = torch.tensor([[n, 0, 1, 2, 3, 130, 0, 0, n - 5]], dtype=torch.int32, device="cuda")
+    mass = torch.rand(1, h, cap, generator=g, device="cuda")
+    pos = torch.arange(cap, dtype=torch.int32, device="cuda").expand(1, h, cap).contiguous()
+    cache = KVCache(k, v, lengths, mass, pos)
+    q, kn, vn = (torch.randn(1, t, h, d, generator=gen).to(torch.bfloat16).cuda().transpose(1, 2) for _ in range(3))
+    out, lse = tree_attention(q, kn, vn, cache)
+    want = mass.clone()
+    for head in (0, 5, 8):
+        m = int(lengths[0, head])
+        keys, values = torch.cat([k[0, head, :m], kn[0, head]]).double(), torch.cat([v[0, head, :m], vn[0, head]]).double()
+        x = q[0, head].double() @ keys.T * d ** -0.5
+        x[0, -1] = -math.inf  # a chain: the first draft does not see the second
+        ref_lse = torch.logsumexp(x, -1)
+        p = torch.exp(x - ref_lse[:, None])
+        spread = p @ values.abs()
+        assert ((lse[0, head] - ref_lse).abs() <= 1e-5 * ref_lse.abs()).all()
+        assert ((out[0, head].double() - p @ values).abs() <= 2.0 ** -8 * 1.01 * (spread + (p @ values).abs()) + 1e-5 * spread).all()
+        want[0, head, :m] += p[:, :m].sum(0).float()
+        want[0, head, m:m + t] = p[:, m:].sum(0).float()
+    steps = torch.arange(t, dtype=torch.int32, device="cuda")[None]
+    commit_tokens(cache, q, kn, vn, lse, steps, cap + steps)
+    for head in (0, 5, 8):
+        m = int(lengths[0, head])  # the new length
+        torch.testing.assert_close(cache.mass[0, head, :m], want[0, head, :m], rtol=1e-5, atol=1e-9)
+        assert torch.equal(k[0, head, m - t:m], kn[0, head]) and torch.equal(v[0, head, m - t:m], vn[0, head])
+    budget = n - 50
+    old = {head: (cache.mass[0, head].clone(), k[0, head, budget:].clone(), v[0, head, budget:].clone()) for head in (0, 8)}
+    untouched = k[0, 0, :1000].clone(), v[0, 8, 500_000:501_000].clone()
+    evict_tokens(cache, budget, recent=20)
+    for head, (m, k_old, v_old) in old.items():
+        before = n if head == 0 else n - 5
+        places = list(range(before)) + [cap, cap + 1]
+        src = torch.tensor(O.evict_slots(m[:before + t].tolist(), places, budget, 20), device="cuda")
+        moved = (src >= budget).nonzero()[:, 0]
+        assert len(moved) > 0 and int(cache.lengths[0, head]) == budget
+        assert torch.equal(cache.mass[0, head, :budget], m[src])
+        assert torch.equal(k[0, head, moved], k_old[src[moved] - budget]) and torch.equal(v[0, head, moved], v_old[src[moved] - budget])
+    assert (k[0, 0, :1000] != untouched[0]).any(-1).sum() < 10 and (v[0, 8, 500_000:501_000] != untouched[1]).any(-1).sum() < 10
+
+
 # ------------------------------------------------------------------------------ together
 
 
