@@ -45,7 +45,7 @@ class KVCache:
     copied, and cannot be replaced: update them in place.
     """
 
-    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "device", "dtype", "_sync", "_sizes", "_c", "_ref", "_device_index")
+    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "device", "dtype", "_sync", "_sizes", "_over", "_c", "_ref", "_device_index")
 
     def __init__(self, k, v, lengths, mass=None, positions=None, norms=None):
         if k.ndim != 4 or k.shape != v.shape or k.numel() == 0 or k.shape[-1] > 256:
@@ -71,6 +71,7 @@ class KVCache:
                                     lengths.data_ptr(), None, b, h, c, d, _DTYPES[k.dtype]))
         init(self, "_ref", ctypes.byref(self._c))
         init(self, "_sizes", {})  # workspace bytes by the calls' shapes
+        init(self, "_over", None)  # the cache that this one was last checked to be another bookkeeping of
         _lib.check(_lib.load().fe_cache_prepare(self._ref))
         init(self, "device", k.device)
         init(self, "dtype", k.dtype)
@@ -220,6 +221,8 @@ def _check_out(cache, out):
         raise ValueError("the cache has no mass and positions")
     if out is None or out is cache:
         return cache
+    if out._over is cache:  # neither's tensors can have been replaced since
+        return out
     if out.mass is None or (out.norms is None) != (cache.norms is None) or out.mass.data_ptr() == cache.mass.data_ptr() \
             or out.positions.data_ptr() == cache.positions.data_ptr() or out.lengths.data_ptr() == cache.lengths.data_ptr() \
             or (out.norms is not None and out.norms.data_ptr() == cache.norms.data_ptr()):
@@ -227,6 +230,7 @@ def _check_out(cache, out):
     if cache.k.data_ptr() != out.k.data_ptr() or cache.v.data_ptr() != out.v.data_ptr() or cache.k.shape != out.k.shape \
             or cache.k.dtype != out.k.dtype or cache.k.stride() != out.k.stride() or cache.v.stride() != out.v.stride():
         raise ValueError("out must hold the cache's own k and v")
+    object.__setattr__(out, "_over", cache)
     return out
 
 
