@@ -158,10 +158,11 @@ __device__ __noinline__ void tree_add_special(const TreeParams& p, int b, int h,
   }
 }
 
+// Nonzero if one of two packed 16-bit values has all exponent bits set.
 template <bool BF16>
-__device__ __forceinline__ bool not_finite2(uint32_t w) {
-  constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
-  return (w & E) == E || ((w >> 16) & E) == E;
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+  constexpr uint32_t E = BF16 ? 0x7f807f80u : 0x7c007c00u;
+  return __vcmpeq2(w & E, E);
 }
 
 constexpr int TREE_CLUSTER = 8;
@@ -506,27 +507,28 @@ __global__ void __launch_bounds__(384, 1)
             // Clear those rows (thread = V row) before the product reads them.
             ok = warp_all(mbar_wait(&v_full[s], (tile / C::STAGES) & 1, TO, abort_flag));
             if (!ok) break;
+            // (Rows past the drafts were filled with zeros by the load.)
             uint8_t* vt = smem + C::OFF_V + s * C::TILE + r * 128;
-            bool clear = r > lim;
-            if (drafts && !clear) {
-              bool bad = false;
+            bool clear = r > lim && !drafts;
+            if (drafts && r <= lim) {
+              uint32_t bad = 0u;
+#pragma unroll
               for (int c = 0; c < C::NCH; ++c)
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
-                  const uint4 w = *reinterpret_cast<const uint4*>(vt + c * 16384 + ((u ^ (r & 7)) << 4));
-                  bad = bad || not_finite2<BF16>(w.x) || not_finite2<BF16>(w.y) || not_finite2<BF16>(w.z) ||
-                        not_finite2<BF16>(w.w);
+                  const uint4 w = *reinterpret_cast<const uint4*>(vt + c * 16384 + (u << 4));
+                  bad |= not_finite2<BF16>(w.x) | not_finite2<BF16>(w.y) | not_finite2<BF16>(w.z) | not_finite2<BF16>(w.w);
                 }
-              if (bad) atomicOr(&spec[r >> 5], 1u << (r & 31));
-              clear = bad;
+              clear = bad != 0u;
+              if (clear) atomicOr(&spec[r >> 5], 1u << (r & 31));
             }
-            if (clear) {
-              for (int c = 0; c < C::NCH; ++c)
+            if (__any_sync(0xffffffffu, clear)) {
+              for (int c = 0; c < C::NCH && clear; ++c)
 #pragma unroll
                 for (int u = 0; u < 8; ++u)
                   *reinterpret_cast<uint4*>(vt + c * 16384 + ((u ^ (r & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+              fence_proxy_async_smem();
             }
-            fence_proxy_async_smem();
           }
           if (warp_live) {
             float x[128];
