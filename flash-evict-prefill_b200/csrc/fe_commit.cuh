@@ -32,9 +32,6 @@
 namespace fe {
 
 constexpr int COMMIT_MAX_ACCEPTED = 128;
-// Key tiles that beginning a row costs (batch of 16: 35.5 us with none, 33.0 with
-// 2, 32.2 with 3; 5 drafts of 64 over 32k 18.8, 14.8, 16.5).
-constexpr int COMMIT_EXTRA = 2;
 
 struct CommitParams {
   const uint16_t* q;
@@ -64,6 +61,7 @@ struct CommitParams {
   int64_t v_sb, v_sh, v_st;
   const int32_t* new_positions;  // [B, T]
   int B, Hq, Hkv, G, T, A, D, capacity, nctas;
+  int extra;           // key tiles that beginning a row costs
   int row0;            // first query row (i*G + g) of this launch
   int last;            // the last launch: append
   int copy;            // mass_out, norms_out, pos_out are other buffers: fill them
@@ -304,7 +302,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
   }
   tc_fence_before();
   pdl_wait();  // nothing above reads or writes memory
-  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, 1, COMMIT_EXTRA, blockIdx.x, p.nctas,
+  DecWalk walk = dec_walk_init<C::THREADS>(p.lengths, p.B * p.Hkv, p.capacity, 1, p.extra, blockIdx.x, p.nctas,
                                                scratch);
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
@@ -462,24 +460,16 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         const int padded = (rows + 15) & ~15;
         constexpr int CPR = DP / 8;
         const uint16_t* qb = p.q + b * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
-        for (int i0 = tid; wg < C::WGS - 1 && i0 < padded * CPR; i0 += QT * 4) {
-          uint4 v[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * QT;
-            const int r = i / CPR;
-            v[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (r < rows) {
-              const int qi = (p.row0 + r) / p.G, g = p.row0 + r - qi * p.G;
-              v[u] = load_row_chunk(qb + g * p.q_sh + slist[qi] * p.q_st, i % CPR, p.D, p.q_vec);
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int i = i0 + u * QT;
-            const int r = i / CPR;
-            if (r < padded)
-              *reinterpret_cast<uint4*>(smem + C::OFF_Q + (r >> 7) * C::TILE + sw128_offset(r & 127, i % CPR, 16384)) = v[u];
+        for (int i = tid; wg < C::WGS - 1 && i < padded * CPR; i += QT) {
+          const int r = i / CPR, chunk = i % CPR;
+          uint8_t* dst = smem + C::OFF_Q + (r >> 7) * C::TILE + sw128_offset(r & 127, chunk, 16384);
+          const int qi = r < rows ? (p.row0 + r) / p.G : 0, g = r < rows ? p.row0 + r - qi * p.G : 0;
+          const uint16_t* src = qb + g * p.q_sh + slist[qi] * p.q_st;
+          if (p.q_vec) {
+            const bool live = r < rows && chunk * 8 < p.D;
+            cp_async16(dst, live ? src + chunk * 8 : qb, live);
+          } else {
+            *reinterpret_cast<uint4*>(dst) = r < rows ? load_row_chunk(src, chunk, p.D) : make_uint4(0u, 0u, 0u, 0u);
           }
         }
         for (int r = tid - QT; wg == C::WGS - 1 && r < padded; r += 128) {
@@ -513,6 +503,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
             scol[3 * C::ROWS + r] = m.w;
           }
         }
+        cp_async_wait_all();
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);

@@ -136,25 +136,27 @@ __device__ __forceinline__ uint32_t sw128_offset(int r, int chunk, int group_byt
   return static_cast<uint32_t>((chunk >> 3) * group_bytes + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
 }
 
-// Eight consecutive channels of a row of 16-bit elements, zero past `channels`.
-// vec: the row is 16-byte aligned and channels is a multiple of 8.
-__device__ __forceinline__ uint4 load_row_chunk(const uint16_t* row, int chunk, int channels, bool vec) {
-  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+// Eight consecutive channels of a row of 16-bit elements, zero past `channels`,
+// read one by one (rows that are not on 16 bytes).
+__device__ __forceinline__ uint4 load_row_chunk(const uint16_t* row, int chunk, int channels) {
   const int c = chunk * 8;
-  if (vec) {
-    if (c < channels) v = __ldg(reinterpret_cast<const uint4*>(row + c));
-  } else {
-    uint32_t w[4];
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = c + 2 * i < channels ? __ldg(row + c + 2 * i) : 0u;
-      const uint32_t hi = c + 2 * i + 1 < channels ? __ldg(row + c + 2 * i + 1) : 0u;
-      w[i] = lo | (hi << 16);
-    }
-    v = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = c + 2 * i < channels ? __ldg(row + c + 2 * i) : 0u;
+    const uint32_t hi = c + 2 * i + 1 < channels ? __ldg(row + c + 2 * i + 1) : 0u;
+    w[i] = lo | (hi << 16);
   }
-  return v;
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
+
+// Asynchronous 16-byte copy from global to shared memory; live == false fills
+// zeros (src must still be a valid address).
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(live ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Bits of up to 32 mask bytes (1 where nonzero).  vec: 16-byte aligned, n a
 // multiple of 16; otherwise all bytes are loaded before the first is used.
