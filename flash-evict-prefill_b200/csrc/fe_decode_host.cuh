@@ -283,7 +283,6 @@ int fe_tree_attention(const fe_cache* cache, const void* q, const int64_t* q_str
   p.D4 = (int)g.D4;
   p.nctas = (int)g.ctas;
   p.sc = (float)((double)scale * 1.4426950408889634);
-  p.tree_vec = mask_is_vectors(tree, tree_batch_stride, drafts);
   p.timeout_ns = (uint64_t)g_watchdog_ns;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int dp = padded_dim(D);
