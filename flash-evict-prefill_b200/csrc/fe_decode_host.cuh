@@ -158,6 +158,33 @@ int launch_dependent(Kern kern, dim3 grid, dim3 block, int smem, int cluster, cu
   return FE_STATUS_OK;
 }
 
+// Clusters of `ctas` eviction CTAs (one to an SM) that are resident at once: one
+// stays within a GPC, so larger ones leave SMs over (clusters of four use 136 of
+// a B200's 148 SMs, of eight fewer still).
+int64_t resident_rows(int dev, int ctas) {
+  static std::atomic<int> counts[kMaxDevices][fe::SHRINK_MAX_CLUSTER + 1];  // 0: not asked yet
+  if (ctas == 1 || dev < 0 || dev >= kMaxDevices) return sm_count(dev) / ctas;
+  int n = counts[dev][ctas].load(std::memory_order_relaxed);
+  if (n) return n;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(fe::SHRINK_THREADS);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, fe::fe_shrink_kernel<true>, &cfg) != cudaSuccess) {
+    cudaGetLastError();  // (a guess is as right, if slower)
+    n = sm_count(dev) / ctas;
+  }
+  n = std::max(n, 1);
+  counts[dev][ctas].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 template <bool BF16, int DP, bool DUAL, bool CLUSTER>
 int launch_tree(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tkn, const CUtensorMap& tvn,
                 const fe::TreeParams& p, cudaStream_t stream) {
@@ -506,19 +533,23 @@ int fe_evict_tokens(const fe_cache* cache, const fe_cache* out, int64_t budget, 
   p.recent = (int)std::min<int64_t>(recent, 0x7fffffff);
   p.row_bytes = (int)cache->channels * 2;
   p.copy = cache->mass != out->mass;
-  // A second launch for the moves where a row may have more than 1 MB of them
-  // to read and write and the rows use a good part of the SMs; then a row needs
-  // fewer CTAs to select (batch of 16 with 8 heads, budget 4096: 41 -> 36 us).
-  const bool two = list * p.row_bytes * 4 > (int64_t(1) << 20) && rows * 4 >= sm_count(dev);
-  if (two) p.counts = p.movers + rows * list;
-  // CTAs per row: as many as hold the row's keys, and more while they would
-  // still have 2048 keys each and the SMs are not all used.
+  // CTAs per row: as many as hold the row's keys, and, from 8192 slots on (below,
+  // the cluster's barriers cost more: 12.0 us with one CTA, 14.3 with two for 32
+  // rows of 5000), more while they still have 2048 slots each and all rows'
+  // clusters are resident at once (48 rows of 12000: 19.3 us with two, 28.9 with four).
   auto held = [&](int ctas) {
     return round_up((cap + ctas * fe::SHRINK_WARPS - 1) / (ctas * fe::SHRINK_WARPS), 32) * fe::SHRINK_WARPS;
   };
   int cl = 1;
   while (cl < fe::SHRINK_MAX_CLUSTER && held(cl) > fe::SHRINK_SMEM_KEYS) cl *= 2;
-  while (cl < fe::SHRINK_MAX_CLUSTER && rows * cl * (two ? 2 : 1) <= sm_count(dev) && cap / (2 * cl) >= 2048) cl *= 2;
+  while (cl < fe::SHRINK_MAX_CLUSTER && cap >= 8192 && cap / (2 * cl) >= 2048 && rows <= resident_rows(dev, 2 * cl)) cl *= 2;
+  // A second launch for the moves where it may spare the busiest SM 256 KB of
+  // reads and writes: a row's own CTAs share its moves, the launch's all rows'.
+  // (Rows of 46000 to a quarter, four rows 38.7 us in one launch, 25.6 in two, 24
+  // rows 69 and 63; to a 32nd, 64 rows, where it spares less, 48 and 50.)
+  const int64_t sms = sm_count(dev), resident = resident_rows(dev, cl), waves = (rows + resident - 1) / resident;
+  const bool two = list * p.row_bytes * 4 * (waves * sms - rows * cl) >= (int64_t(256) << 10) * cl * sms;
+  if (two) p.counts = p.movers + rows * list;
   const bool smem_keys = held(cl) <= fe::SHRINK_SMEM_KEYS;
   p.hold_positions = smem_keys && recent > 0 && 2 * held(cl) <= fe::SHRINK_SMEM_KEYS;
   auto kern = smem_keys ? fe::fe_shrink_kernel<true> : fe::fe_shrink_kernel<false>;

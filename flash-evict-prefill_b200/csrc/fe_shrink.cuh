@@ -22,8 +22,8 @@
 // ending as soon as a bin's end coincides with the budget (one or two passes for
 // a row of a few thousand).  Holes and movers are numbered by ballots in slot order,
 // listed, and copied by all warps of the cluster, eight rows a warp in flight.
-// Where a CTA might have much to copy, a second launch splits all rows' moves
-// evenly instead (rows need very different numbers of them).  Few rows are bound
+// Where that leaves some SM much more to copy than others (few rows, rows with
+// very different numbers of moves), a second launch splits all rows' moves evenly.  Few rows are bound
 // by the chain of cluster barriers, large batches by the moved bytes.
 #pragma once
 

@@ -248,6 +248,22 @@ def test_evict_many_rows_with_much_to_move():
     check_evict(cache, 1449, 0)
 
 
+@pytest.mark.parametrize("rows, cap, budget, recent", [
+    (3, 2300, 1100, 64),     # one CTA a row, moves in a launch of their own
+    (3, 8300, 4000, 0),      # small clusters, and the same
+    (2, 33000, 9000, 100),   # large ones
+    (20, 17000, 260, 0),     # clusters of four, which move the rows themselves
+    (70, 8300, 300, 20),     # of two
+    (80, 8300, 200, 0),      # too many rows for clusters
+])
+def test_evict_launch_shapes(rows, cap, budget, recent):
+    gen = torch.Generator().manual_seed(rows + cap)
+    lengths = torch.randint(budget - 50, cap + 1, (1, rows), generator=gen)
+    lengths[0, 0], lengths[0, -1] = cap, budget + 1
+    cache, _ = cache_for_eviction(39, 1, rows, 96, cap, lengths.tolist())
+    check_evict(cache, budget, recent)
+
+
 def test_evict_ties_zeros_infinities_and_nan():
     cache, gen = cache_for_eviction(34, 1, 4, 32, 3000, 3000)
     m = cache.mass
