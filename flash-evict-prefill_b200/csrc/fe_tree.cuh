@@ -333,6 +333,7 @@ __global__ void __launch_bounds__(384, 1)
     const int share = (tiles + TREE_CLUSTER - 1) / TREE_CLUSTER, j0 = min(rank * share, tiles);
     walk.left = min(share, tiles - j0);
     walk.unit = (item - walk.bh * p.MT) * tiles + j0;
+    if (threadIdx.x == 0) scratch[0] = (tiles + share - 1) / share;  // CTAs that have tiles
     __syncthreads();
   } else {
     // Ends with a block barrier, which also publishes the barriers and TMEM.
@@ -688,8 +689,7 @@ __global__ void __launch_bounds__(384, 1)
       const float4* s_part = reinterpret_cast<const float4*>(smem);
       const int item = blockIdx.x / TREE_CLUSTER, rank = blockIdx.x % TREE_CLUSTER;
       const int bh = item / p.MT, mt = item - bh * p.MT;
-      const int tiles = (cache_length(p.lengths, bh, p.capacity) + DEC_TILE - 1) / DEC_TILE + 1;
-      const int share_t = (tiles + TREE_CLUSTER - 1) / TREE_CLUSTER, used = (tiles + share_t - 1) / share_t;
+      const int used = scratch[0];
       const int rows = min(p.M - mt * p.tile_rows, p.tile_rows), pairs = rows * (p.D4 / 4);
       const int share = (pairs + TREE_CLUSTER - 1) / TREE_CLUSTER, end = min(pairs, (rank + 1) * share);
       for (int i = rank * share + static_cast<int>(threadIdx.x); i < end; i += 256) {
