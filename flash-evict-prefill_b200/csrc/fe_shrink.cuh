@@ -23,8 +23,9 @@
 // a row of a few thousand).  Holes and movers are numbered by ballots in slot order,
 // listed, and copied by all warps of the cluster, eight rows a warp in flight.
 // Where that leaves some SM much more to copy than others (few rows, rows with
-// very different numbers of moves), a second launch splits all rows' moves evenly.  Few rows are bound
-// by the chain of cluster barriers, large batches by the moved bytes.
+// very different numbers of moves), a second launch splits all rows' moves evenly.
+// Few rows are bound by the chain of cluster barriers, large batches by the moved
+// bytes.
 #pragma once
 
 #include <cooperative_groups.h>
