@@ -14,13 +14,10 @@ weight (mass), the L1 norm of its value row (norms) and the token's position.  T
 pass is written beside the old one (`out=`), so a pass can be repeated.
 """
 import math
-import os
-import sys
 
 import torch
 
 own = False
-PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "flash-evict-prefill_b200")
 
 DTYPES = {"float16": torch.float16, "bfloat16": torch.bfloat16}
 
@@ -154,8 +151,6 @@ def prepare(case, seed):
         if case["kind"] == "commit":
             s["lse"] = _plain_attend(s)[1]
     if own:
-        if PACKAGE not in sys.path:
-            sys.path.insert(0, PACKAGE)
         from flash_evict.decode import KVCache
         s["cache"] = KVCache(k, v, **book)
         s["out_cache"] = KVCache(k, v, **s["out"])
