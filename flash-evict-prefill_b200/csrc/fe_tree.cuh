@@ -747,7 +747,10 @@ __global__ void __launch_bounds__(TREE_JOIN_THREADS)
   const int pair = (blockIdx.y * (TREE_JOIN_WARPS / splits) + warp / splits) * 32 + lane;
   const bool live = pair < rows * groups;
   const int quad0 = live ? pair / rows * Q : 0, r = live ? pair % rows : 0;
-  // Which runs had the row: from the lengths alone, before the runs are done.
+  // Which runs had the row.  (The kernel before the attention may have written
+  // the lengths and still be running until here: the attention lets this one
+  // start ahead of its own wait.)
+  pdl_wait();
   int first, last, start;
   const DecLayout d = dec_layout<TREE_JOIN_THREADS>(p.lengths, p.B * p.Hkv, p.capacity, p.MT, TREE_EXTRA, p.nctas, scratch,
                                                     first, last, start);
@@ -759,7 +762,6 @@ __global__ void __launch_bounds__(TREE_JOIN_THREADS)
   const int tiles = (cache_length(p.lengths, bh, p.capacity) + DEC_TILE - 1) / DEC_TILE + 1;
   const int u0 = s_start + mt * (tiles + d.extra);
   const int c0 = u0 / d.per, n = (u0 + tiles - 1) / d.per - c0 + 1;
-  pdl_wait();
   if (n == 1) return;  // one run had the whole row and wrote it
   const int64_t slot0 = static_cast<int64_t>(item) + c0;
   const float2* st_row = p.stats + slot0 * p.R + r;

@@ -1,0 +1,75 @@
+"""Decode operators back to back, as a captured step runs them, against the same calls one at a time.
+
+Every kernel may start while the ones before it end, so whatever a call reads of
+the cache has to be what the call before it wrote.  The results are compared bit
+by bit: the operators are reproducible, and only the timing differs.
+"""
+import pytest
+import torch
+
+from flash_evict.decode import commit_tokens, evict_tokens, tree_attention
+from test_gpu_decode import make, random_tree
+from test_gpu_decode_cache import bits, clone, path_of, with_book
+
+pytestmark = pytest.mark.gpu
+
+
+def same(a, b):
+    """The live tokens and lengths of two caches."""
+    assert torch.equal(a.lengths, b.lengths)
+    live = torch.arange(a.k.shape[2], device="cuda") < a.lengths[..., None]
+    for x, y in ((a.k, b.k), (a.v, b.v), (a.mass, b.mass), (a.norms, b.norms), (a.positions, b.positions)):
+        assert torch.equal(bits(x)[live], bits(y)[live])
+
+
+# Attentions whose runs leave SMs free (so that the join of the runs can be
+# resident early), with lengths that change the number of key tiles at every step.
+SHAPES = [
+    # b, hq, hk, d, budget, spare, t, accepted
+    (1, 32, 8, 128, 1024, 128, 64, 5),
+    (1, 28, 4, 128, 1024, 128, 64, 5),
+    (1, 8, 1, 128, 8192, 128, 1, 1),
+    (1, 4, 4, 128, 4352, 128, 1, 1),
+    (4, 8, 8, 64, 256, 128, 1, 1),
+]
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention_right_after_a_change_of_the_lengths(shape):
+    b, hq, hk, d, budget, spare, t, took = shape
+    q, kn, vn, cache, gen = make(sum(shape), b, hq, hk, d, budget + spare, t, torch.bfloat16, budget + took, junk=0.0)
+    cache = with_book(cache, gen)
+    tree = random_tree(gen, 1, t)[0]
+    path = path_of(tree, took)
+    path = path + [j for j in range(t) if j not in path][:took - len(path)]
+    accepted = torch.tensor([path], dtype=torch.int32).expand(b, took).contiguous().cuda()
+    positions = torch.full((b, t), 10 ** 6, dtype=torch.int32, device="cuda")
+    tree = tree.cuda() if t > 1 else None
+    plain = clone(cache)
+
+    def steps(c, between):
+        got = []
+        for _ in range(4):
+            evict_tokens(c, budget, recent=8)
+            between()
+            got.append(tree_attention(q, kn, vn, c, tree=tree))
+            between()
+            commit_tokens(c, q, kn, vn, got[-1][1], accepted, positions, tree=tree)
+            between()
+            got.append(tree_attention(q, kn, vn, c, tree=tree))
+            between()
+        return got
+
+    want = steps(plain, torch.cuda.synchronize)
+    steps(clone(cache), torch.cuda.synchronize)
+    graph = torch.cuda.CUDAGraph()
+    start = clone(cache)
+    with torch.cuda.graph(graph):
+        got = steps(cache, lambda: None)
+    for _ in range(5):
+        for name in ("k", "v", "mass", "norms", "positions", "lengths"):
+            getattr(cache, name).copy_(getattr(start, name))
+        graph.replay()
+        for (out, lse), (ref, ref_lse) in zip(got, want):
+            assert torch.equal(bits(lse), bits(ref_lse)) and torch.equal(bits(out), bits(ref))
+        same(cache, plain)
