@@ -88,9 +88,10 @@ constexpr int TREE_EXTRA = 3;
 constexpr uint32_t TREE_QBUF = 8192;  // bytes between the halves of a query tile's 64-column group
 
 // One key tile of a row's softmax (S in x).  With `masked`, only columns with
-// their bit set count.
+// their bit set count.  Lanes that hold no query (!live) have scores of whatever
+// lay in the query tile: they follow the warp's rescaling and have no say in it.
 template <bool BF16, int DV>
-__device__ __forceinline__ void tree_softmax_tile(float (&x)[128], bool first, bool masked, const uint32_t (&bits)[4],
+__device__ __forceinline__ void tree_softmax_tile(float (&x)[128], bool live, bool first, bool masked, const uint32_t (&bits)[4],
                                                   float sc, float sce, bool sc_pos, float& m_used, float& l,
                                                   uint32_t tS, uint32_t tO) {
   if (!sc_pos) {
@@ -104,7 +105,7 @@ __device__ __forceinline__ void tree_softmax_tile(float (&x)[128], bool first, b
   const float m_new = fmaxf(m_used, row_max_scaled(x, sce));
   if (first) {
     m_used = m_new;
-  } else if (__any_sync(0xffffffffu, m_new > m_used + FWD_RESCALE_LOG2)) {
+  } else if (__any_sync(0xffffffffu, live && m_new > m_used + FWD_RESCALE_LOG2)) {
     // The product that last wrote O completed before this S did.
     const float f = ex2_approx(m_used - m_new);
     l *= f;
@@ -580,9 +581,9 @@ __global__ void __launch_bounds__(384, 1)
             }
             const bool masked = drafts || lim < 127;
             if (DUAL && !masked)  // the long runs' loop, free of masking code
-              tree_softmax_tile<BF16, DP>(x, first, false, sees, sc, sce, sc_pos, m_used, l, tS, tO);
+              tree_softmax_tile<BF16, DP>(x, live, first, false, sees, sc, sce, sc_pos, m_used, l, tS, tO);
             else
-              tree_softmax_tile<BF16, DP>(x, first, masked, sees, sc, sce, sc_pos, m_used, l, tS, tO);
+              tree_softmax_tile<BF16, DP>(x, live, first, masked, sees, sc, sce, sc_pos, m_used, l, tS, tO);
           }
           first = false;
           tc_fence_before();

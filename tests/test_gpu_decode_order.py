@@ -31,6 +31,7 @@ SHAPES = [
     (1, 8, 1, 128, 8192, 128, 1, 1),
     (1, 4, 4, 128, 4352, 128, 1, 1),
     (4, 8, 8, 64, 256, 128, 1, 1),
+    (2, 8, 4, 256, 1024, 100, 3, 2),  # (a cluster a row)
 ]
 
 
@@ -73,3 +74,18 @@ def test_attention_right_after_a_change_of_the_lengths(shape):
         for (out, lse), (ref, ref_lse) in zip(got, want):
             assert torch.equal(bits(lse), bits(ref_lse)) and torch.equal(bits(out), bits(ref))
         same(cache, plain)
+
+
+@pytest.mark.parametrize("b,hq,hk,d,n,dtype", [(1, 28, 4, 128, 2048, torch.float16), (1, 28, 4, 128, 20000, torch.bfloat16),
+                                               (16, 14, 2, 64, 3000, torch.bfloat16), (1, 6, 2, 256, 3000, torch.float16)])
+def test_what_ran_before_leaves_no_trace(b, hq, hk, d, n, dtype):
+    # Queries fill a part of their tile; the rest holds what an earlier kernel left
+    # in shared memory, here the queries of a call with full tiles.
+    q, kn, vn, cache, _ = make(51, b, hq, hk, d, n + 64, 1, dtype, n, sharp=2.0)
+    full, fk, fv, _, _ = make(52, b, 8 * hk, hk, d, 64, 16, dtype, 0)
+    seen = []
+    for loud in (0.0, 30.0, 1000.0, 0.0):
+        tree_attention(full * loud, fk, fv, cache)
+        seen.append(tree_attention(q, kn, vn, cache))
+    for out, lse in seen[1:]:
+        assert torch.equal(bits(out), bits(seen[0][0])) and torch.equal(bits(lse), bits(seen[0][1]))
