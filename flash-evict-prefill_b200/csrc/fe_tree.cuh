@@ -520,8 +520,11 @@ __global__ void __launch_bounds__(384, 1)
           // after its O, whose last product is issued after this group's first P.
           tree_bits<DUAL ? 8 : 4>(p, b, tt, DUAL ? warp : warp & 3, DUAL ? 3 : 1 + t, reinterpret_cast<uint2*>(s_ml), bits);
           if (!live) bits[0] = bits[1] = bits[2] = bits[3] = 0u;
+          // Nobody reads this list any more: two segments back, both groups of two
+          // query tiles did (SPLIT's groups meet at every segment's end).
+          if constexpr (DUAL) named_bar_sync(3, 256);
           if (t == owner) {
-            named_bar_sync(1 + t, 128);
+            if constexpr (!DUAL) named_bar_sync(1 + t, 128);
             if (r < 4) spec[r] = 0u;
             named_bar_sync(1 + t, 128);
           }

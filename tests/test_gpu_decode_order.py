@@ -89,3 +89,20 @@ def test_what_ran_before_leaves_no_trace(b, hq, hk, d, n, dtype):
         seen.append(tree_attention(q, kn, vn, cache))
     for out, lse in seen[1:]:
         assert torch.equal(bits(out), bits(seen[0][0])) and torch.equal(bits(lse), bits(seen[0][1]))
+
+
+@pytest.mark.parametrize("t,group,d", [(100, 2, 64), (37, 7, 128), (128, 3, 128)])
+def test_drafts_without_a_mask_over_many_rows_two_query_tiles_each(t, group, d):
+    # Empty rows are single tiles, through which the two warpgroups of a run pass
+    # at their own pace; which drafts' values are not finite is noted per row.
+    b, hk, cap = 48, 8, 400
+    gen = torch.Generator().manual_seed(t)
+    lengths = (torch.randint(0, 4, (b, hk), generator=gen) == 0) * torch.randint(0, cap, (b, hk), generator=gen)
+    q, kn, vn, cache, _ = make(53, b, group * hk, hk, d, cap, t, torch.bfloat16, lengths.tolist())
+    bad = torch.rand(b, hk, t, d, generator=gen) < 2e-4
+    vn = torch.where(bad.cuda(), torch.inf, vn.float()).to(vn.dtype)
+    # a chain: a draft sees the ones before it and itself
+    want = bad.cumsum(2).bool().repeat_interleave(group, 1).cuda()
+    for _ in range(5):
+        out, lse = tree_attention(q, kn, vn, cache)
+        assert torch.equal(torch.isposinf(out), want) and torch.equal(torch.isfinite(out), ~want) and torch.isfinite(lse).all()
