@@ -111,7 +111,7 @@ __device__ __forceinline__ int accepted_drafts(const int32_t* accepted, int A, i
   const int lane = threadIdx.x & 31;
   int n = 0;
   for (int a0 = 0; a0 < A; a0 += 32) {
-    const int j = a0 + lane < A ? __ldg(accepted + static_cast<int64_t>(b) * A + a0 + lane) : -1;
+    const int j = a0 + lane < A ? accepted[static_cast<int64_t>(b) * A + a0 + lane] : -1;
     const bool valid = j >= 0 && j < T;
     const uint32_t bal = __ballot_sync(0xffffffffu, valid);
     if (valid && list != nullptr) list[n + __popc(bal & ((1u << lane) - 1u))] = j;
@@ -239,7 +239,7 @@ __device__ __forceinline__ void commit_append_rows(const CommitParams& p, int bh
         const int64_t at = base + len + i0 + u;
         if (p.norms_out != nullptr) p.norms_out[at] = norm[u];
         norms[i0 + u] = p.norms_out != nullptr ? norm[u] : 1.0f;
-        p.pos_out[at] = __ldg(p.new_positions + static_cast<int64_t>(b) * p.T + list[i0 + u]);
+        p.pos_out[at] = p.new_positions[static_cast<int64_t>(b) * p.T + list[i0 + u]];
       }
     }
   }
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
       if (w == 0) {
         bool bad = false;
         if (h == 0)
-          for (int a = lane; a < p.A; a += 32) bad = bad || __ldg(p.accepted + static_cast<int64_t>(b) * p.A + a) >= p.T;
+          for (int a = lane; a < p.A; a += 32) bad = bad || p.accepted[static_cast<int64_t>(b) * p.A + a] >= p.T;
         if (bad) raise_status(FE_STATUS_BAD_INDEX);
         if (lane == 0) {
           p.new_lengths[sg.bh] = sg.len + fit;
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
           float bias = -INFINITY;  // padding, and rows that saw nothing, add 0
           if (r < rows) {
             const int qi = (p.row0 + r) / p.G, g = p.row0 + r - qi * p.G;
-            const float lse = __ldg(p.lse + (static_cast<int64_t>(b) * p.Hq + h * p.G + g) * p.T + slist[qi]);
+            const float lse = p.lse[(static_cast<int64_t>(b) * p.Hq + h * p.G + g) * p.T + slist[qi]];
             // Formed in 64 bits and rounded once: the rounding of its two terms
             // would be up to 1e-6 of a weight each.
             if (lse != -INFINITY)
@@ -519,10 +519,10 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         const int64_t at_new = static_cast<int64_t>(sg.bh) * p.T + kr;
         float mass = 0.f, norm = 1.f;
         if (live && !drafts) {
-          mass = p.row0 == 0 ? __ldg(p.mass_in + at) : p.mass_out[at];
-          if (p.norms_in != nullptr) norm = __ldg(p.norms_in + at);
+          mass = p.row0 == 0 ? p.mass_in[at] : p.mass_out[at];
+          if (p.norms_in != nullptr) norm = p.norms_in[at];
           if (p.copy && p.row0 == 0) {
-            p.pos_out[at] = __ldg(p.pos_in + at);
+            p.pos_out[at] = p.pos_in[at];
             if (p.norms_out != nullptr) p.norms_out[at] = norm;
           }
         } else if (live && p.row0 > 0) {

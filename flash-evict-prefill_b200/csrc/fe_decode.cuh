@@ -16,7 +16,7 @@ namespace fe {
 constexpr int DEC_TILE = 128;  // keys per tile
 
 __device__ __forceinline__ int cache_length(const int32_t* lengths, int bh, int capacity) {
-  return min(max(__ldg(lengths + bh), 0), capacity);
+  return min(max(lengths[bh], 0), capacity);
 }
 
 // One contiguous run of a row's tiles: tiles [j0, j1) of `tiles` for row tile mt.
@@ -143,8 +143,8 @@ __device__ __forceinline__ uint4 load_row_chunk(const uint16_t* row, int chunk, 
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = c + 2 * i < channels ? __ldg(row + c + 2 * i) : 0u;
-    const uint32_t hi = c + 2 * i + 1 < channels ? __ldg(row + c + 2 * i + 1) : 0u;
+    const uint32_t lo = c + 2 * i < channels ? row[c + 2 * i] : 0u;
+    const uint32_t hi = c + 2 * i + 1 < channels ? row[c + 2 * i + 1] : 0u;
     w[i] = lo | (hi << 16);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
@@ -166,7 +166,7 @@ __device__ __forceinline__ uint32_t mask_word(const uint8_t* row, int n, bool ve
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (16 * u >= n) continue;
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(row) + u);
+      const uint4 x = reinterpret_cast<const uint4*>(row)[u];
       // Four mask bytes to four bits: 1 where nonzero, gathered by a multiply.
       v |= ((__vsetgtu4(x.x, 0u) * 0x01020408u) >> 24) << (16 * u);
       v |= ((__vsetgtu4(x.y, 0u) * 0x01020408u) >> 24) << (16 * u + 4);
@@ -176,7 +176,7 @@ __device__ __forceinline__ uint32_t mask_word(const uint8_t* row, int n, bool ve
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (j < n) v |= (__ldg(row + j) != 0 ? 1u : 0u) << j;
+      if (j < n) v |= (row[j] != 0 ? 1u : 0u) << j;
   }
   return v;
 }
@@ -194,7 +194,10 @@ __device__ __forceinline__ float elem_to_float(uint16_t x) {
 // prologue only), and wait until the previous ones are done and their writes
 // are seen.  Every decode kernel is launched so and touches no memory before the
 // wait, so whatever ran before it, decode kernel or not, it only overlaps that
-// one's tail with its own start (barriers, TMEM, descriptors).
+// one's tail with its own start (barriers, TMEM, descriptors).  What they read is
+// therefore not constant while they are resident, and a commit in place writes what
+// it reads: none of it goes through the read-only path (__ldg), whose loads may
+// also be moved ahead of the wait.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -134,7 +134,7 @@ __device__ __forceinline__ void tree_softmax_tile(float (&x)[128], bool live, bo
 // warp.  A lane reads one byte.
 __device__ __forceinline__ uint32_t tree_word(const uint8_t* row, int n) {
   const int lane = threadIdx.x & 31;
-  const bool see = lane < n && __ldg(row + lane) != 0;
+  const bool see = lane < n && row[lane] != 0;
   return __ballot_sync(0xffffffffu, see);
 }
 
