@@ -66,7 +66,7 @@ class KVCache:
             init(self, name, t)
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         b, h, c, d = k.shape
-        init(self, "_sync", None)  # made by the first commit in place
+        init(self, "_sync", None)  # made by the first commit in place outside a capture
         init(self, "_c", _lib.Cache(k.data_ptr(), v.data_ptr(), k.stride(), v.stride(), ptr(mass), ptr(norms), ptr(positions),
                                     lengths.data_ptr(), None, b, h, c, d, _DTYPES[k.dtype]))
         init(self, "_ref", ctypes.byref(self._c))
@@ -81,9 +81,14 @@ class KVCache:
         raise AttributeError("a KVCache's tensors cannot be replaced; update them in place")
 
     def _make_sync(self):
-        # The word that counts a commit's CTAs: zero before and after.
-        object.__setattr__(self, "_sync", torch.zeros(1, dtype=torch.int32, device=self.device))
-        self._c.sync = self._sync.data_ptr()
+        # The word that counts a commit's CTAs: zero before and after.  Under capture it
+        # is zeroed by the graph only, so the graph has one of its own and the cache none.
+        word = torch.zeros(1, dtype=torch.int32, device=self.device)
+        with torch.cuda.device(self.device):
+            if not torch.cuda.is_current_stream_capturing():
+                object.__setattr__(self, "_sync", word)
+        self._c.sync = word.data_ptr()
+        return word
 
     @classmethod
     def allocate(cls, batch, kv_heads, capacity, channels, dtype=torch.bfloat16, device="cuda", *, value_weighted=True):
@@ -268,8 +273,7 @@ def commit_tokens(cache, q, k_new, v_new, lse, accepted, positions, *, tree=None
     recency_decay = float(recency_decay)
     if not math.isfinite(recency_decay) or recency_decay < 0:
         raise ValueError("recency_decay must be finite and nonnegative")
-    if out is cache and cache._sync is None:
-        cache._make_sync()
+    sync = cache._make_sync() if out is cache and cache._sync is None else None  # (kept until the launch)
     lib = _lib.load()
     a = accepted.shape[1]
     size, workspace, pointer = _workspace(cache, (hq, t, a, out is cache), lib.fe_commit_workspace_bytes, cache._ref, out._ref, hq, t, a)

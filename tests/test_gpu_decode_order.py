@@ -106,3 +106,34 @@ def test_drafts_without_a_mask_over_many_rows_two_query_tiles_each(t, group, d):
     for _ in range(5):
         out, lse = tree_attention(q, kn, vn, cache)
         assert torch.equal(torch.isposinf(out), want) and torch.equal(torch.isfinite(out), ~want) and torch.isfinite(lse).all()
+
+
+def test_a_captured_first_commit_leaves_the_cache_ready_for_others():
+    """The first commit of a cache captured and not yet replayed: eager commits and other graphs count their CTAs all the same."""
+    q, kn, vn, cache, gen = make(54, 1, 4, 2, 64, 300, 2, torch.bfloat16, [[250, 0]], junk=0.0)
+    cache = with_book(cache, gen)
+    _, lse = tree_attention(q, kn, vn, cache)
+    accepted = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    positions = torch.tensor([[1000, 1001]], dtype=torch.int32, device="cuda")
+    pool = torch.cuda.graph_pool_handle()
+    before = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(before, pool=pool):
+        junk = [torch.full((128,), 7, dtype=torch.int32, device="cuda") for _ in range(8)]
+    before.replay()  # memory of the pool that holds no zeros
+    del junk
+    plain = clone(cache)
+
+    def commit(c):
+        commit_tokens(c, q, kn, vn, lse, accepted, positions)
+
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph in graphs:
+        with torch.cuda.graph(graph, pool=pool):
+            commit(cache)
+    n = 0
+    for step in (lambda: commit(cache), graphs[1].replay, lambda: commit(cache), graphs[0].replay, graphs[1].replay):
+        step()
+        commit(plain)
+        n += 2
+        assert cache.lengths.tolist() == [[250 + n, n]]
+        same(cache, plain)
