@@ -17,6 +17,7 @@ on the device, so a step can be captured in a CUDA graph):
 import ctypes
 import functools
 import math
+import weakref
 
 import torch
 
@@ -45,7 +46,8 @@ class KVCache:
     copied, and cannot be replaced: update them in place.
     """
 
-    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "device", "dtype", "_sync", "_sizes", "_over", "_c", "_ref", "_device_index")
+    __slots__ = ("k", "v", "lengths", "mass", "positions", "norms", "device", "dtype", "_sync", "_sizes", "_over", "_c", "_ref",
+                 "_device_index", "__weakref__")
 
     def __init__(self, k, v, lengths, mass=None, positions=None, norms=None):
         if k.ndim != 4 or k.shape != v.shape or k.numel() == 0 or k.shape[-1] > 256:
@@ -71,7 +73,7 @@ class KVCache:
                                     lengths.data_ptr(), None, b, h, c, d, _DTYPES[k.dtype]))
         init(self, "_ref", ctypes.byref(self._c))
         init(self, "_sizes", {})  # workspace bytes by the calls' shapes
-        init(self, "_over", None)  # the cache that this one was last checked to be another bookkeeping of
+        init(self, "_over", lambda: None)  # gives the cache that this one was last checked to be another bookkeeping of
         _lib.check(_lib.load().fe_cache_prepare(self._ref))
         init(self, "device", k.device)
         init(self, "dtype", k.dtype)
@@ -226,7 +228,7 @@ def _check_out(cache, out):
         raise ValueError("the cache has no mass and positions")
     if out is None or out is cache:
         return cache
-    if out._over is cache:  # neither's tensors can have been replaced since
+    if out._over() is cache:  # neither's tensors can have been replaced since
         return out
     if out.mass is None or (out.norms is None) != (cache.norms is None) or out.mass.data_ptr() == cache.mass.data_ptr() \
             or out.positions.data_ptr() == cache.positions.data_ptr() or out.lengths.data_ptr() == cache.lengths.data_ptr() \
@@ -235,7 +237,7 @@ def _check_out(cache, out):
     if cache.k.data_ptr() != out.k.data_ptr() or cache.v.data_ptr() != out.v.data_ptr() or cache.k.shape != out.k.shape \
             or cache.k.dtype != out.k.dtype or cache.k.stride() != out.k.stride() or cache.v.stride() != out.v.stride():
         raise ValueError("out must hold the cache's own k and v")
-    object.__setattr__(out, "_over", cache)
+    object.__setattr__(out, "_over", weakref.ref(cache))
     return out
 
 
