@@ -79,6 +79,15 @@ struct TreeCfg {
   static constexpr int THREADS = 384;
 };
 
+// The running maximum m is kept this far below the largest score (in powers of
+// two), so P = 2^(s - m) is at most 2^(8 + 7) with the rescaling's slack.  In fp16
+// that moves the weights that vanish, those under 2^-25, from 2^-25 of the row's
+// largest to 2^-32: together below the output's own rounding for rows of up to 2^20
+// tokens.  O, l and m carry the factor alike, so nothing else knows of it.  (bf16
+// has FP32's range.)
+template <bool BF16>
+constexpr float TREE_HEADROOM = BF16 ? 0.0f : 7.0f;
+
 // Lowest running max: finite, so that a row which has seen no key yet rescales
 // by 2^-huge = 0 and never forms inf - inf.
 constexpr float TREE_M0 = -3.0e38f;
@@ -102,7 +111,7 @@ __device__ __forceinline__ void tree_softmax_tile(float (&x)[128], bool live, bo
 #pragma unroll
     for (int c = 0; c < 128; ++c) x[c] = ((bits[c >> 5] >> (c & 31)) & 1u) ? x[c] : -INFINITY;
   }
-  const float m_new = fmaxf(m_used, row_max_scaled(x, sce));
+  const float m_new = fmaxf(m_used, row_max_scaled(x, sce) - TREE_HEADROOM<BF16>);
   if (first) {
     m_used = m_new;
   } else if (__any_sync(0xffffffffu, live && m_new > m_used + FWD_RESCALE_LOG2)) {
@@ -123,7 +132,8 @@ __device__ __forceinline__ void tree_softmax_tile(float (&x)[128], bool live, bo
   uint32_t pk[64];
   float amax;
   // P is rounded to the input type for the PV product (l sums it unrounded):
-  // its error is that of one rounding per term, below the output's own.
+  // its error is that of one rounding per term, below the output's own, and in
+  // fp16 at most 2^-32 of the row's largest weight where that is more.
   l += softmax_exp_pass<BF16, 0, false, 0>(x, sce, m_used, pk, amax);
   tmem_st32(tS, pk);
   tmem_st32(tS + 32, pk + 32);
