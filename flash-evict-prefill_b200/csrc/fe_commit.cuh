@@ -463,13 +463,15 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         for (int i = tid; wg < C::WGS - 1 && i < padded * CPR; i += QT) {
           const int r = i / CPR, chunk = i % CPR;
           uint8_t* dst = smem + C::OFF_Q + (r >> 7) * C::TILE + sw128_offset(r & 127, chunk, 16384);
-          const int qi = r < rows ? (p.row0 + r) / p.G : 0, g = r < rows ? p.row0 + r - qi * p.G : 0;
+          // (Padding repeats the launch's first query: a score of zeros would be NaN
+          // for a key that is not finite, where that query's may be -inf and add 0.)
+          const int row = p.row0 + (r < rows ? r : 0), qi = row / p.G, g = row - qi * p.G;
           const uint16_t* src = qb + g * p.q_sh + slist[qi] * p.q_st;
           if (p.q_vec) {
-            const bool live = r < rows && chunk * 8 < p.D;
+            const bool live = chunk * 8 < p.D;
             cp_async16(dst, live ? src + chunk * 8 : qb, live);
           } else {
-            *reinterpret_cast<uint4*>(dst) = r < rows ? load_row_chunk(src, chunk, p.D) : make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(dst) = load_row_chunk(src, chunk, p.D);
           }
         }
         for (int r = tid - QT; wg == C::WGS - 1 && r < padded; r += 128) {
