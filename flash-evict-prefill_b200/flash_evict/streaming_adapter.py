@@ -106,12 +106,15 @@ class StreamingController:
     def draft(self, tree):
         """Make the next call's tokens drafts: token t sees the cache and the drafts j with ``tree[t, j]`` (bool [T, T]).
 
-        Nothing is appended until ``accept``.  Give the call ``position_ids`` by depth in the tree.
+        Nothing is appended until ``accept``; drafts of an earlier tree that were not accepted are dropped.  Give the call
+        ``position_ids`` by depth in the tree.
         """
         if self.decode_budget is None or self.mode != "decode":
             raise ValueError("Drafts need decode_budget and decode mode")
         if tree.ndim != 2 or tree.shape[0] != tree.shape[1] or not 1 <= tree.shape[0] <= MAX_DRAFTS or tree.dtype != torch.bool:
             raise ValueError(f"tree must be a bool matrix of 1 to {MAX_DRAFTS} drafts")
+        for state in self.states.values():
+            state.pop("drafts", None)
         self.tree = tree
 
     def accept(self, path):
