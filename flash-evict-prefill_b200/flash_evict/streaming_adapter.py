@@ -30,7 +30,7 @@ those pieces itself:
   tokens attend with ``tree_attention``, add their attention weight to the kept
   tokens and are appended (``commit_tokens``), and the cache is cut back to
   ``decode_budget`` by weight, the newest ``reserved_recent`` tokens excepted
-  (``evict_tokens``).  For speculative decoding, ``draft(tree)`` makes the next
+  (``evict_tokens``); calls of more than 128 tokens go in parts of 128.  For speculative decoding, ``draft(tree)`` makes the next
   call's tokens a tree of drafts that are not appended until
   ``accept(path)`` names the ones to keep.
 
@@ -209,14 +209,19 @@ def _commit(ctl, state, q, k, v, lse, accepted, tree=None):
 def _budgeted_attention(ctl, state, q, k, v, scale):
     state["scale"] = scale
     t = q.shape[2]
-    if ctl.tree is not None and ctl.tree.shape[0] != t:
-        raise ValueError("The call's tokens are not the tree's drafts")
-    out, lse = tree_attention(q, k, v, state["cache"], tree=ctl.tree, scale=scale)
     if ctl.tree is not None:
+        if ctl.tree.shape[0] != t:
+            raise ValueError("The call's tokens are not the tree's drafts")
+        out, lse = tree_attention(q, k, v, state["cache"], tree=ctl.tree, scale=scale)
         state["drafts"] = (q, k, v, lse)
-    else:
-        _commit(ctl, state, q, k, v, lse, torch.arange(t, dtype=torch.int32, device=q.device)[None])
-    return out
+        return out
+    parts = []
+    for at in range(0, t, MAX_DRAFTS):  # each part attends to the cache that the one before left
+        part = [x[:, :, at:at + MAX_DRAFTS] for x in (q, k, v)]
+        out, lse = tree_attention(*part, state["cache"], tree=None, scale=scale)
+        _commit(ctl, state, *part, lse, torch.arange(part[0].shape[2], dtype=torch.int32, device=q.device)[None])
+        parts.append(out)
+    return parts[0] if len(parts) == 1 else torch.cat(parts, 2)
 
 
 def _forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
