@@ -306,6 +306,8 @@ def evict_tokens(cache, budget, *, recent=0, out=None):
         raise ValueError("budget must be a positive integer")
     if isinstance(recent, bool) or not isinstance(recent, int) or not 0 <= recent <= budget:
         raise ValueError("recent must be an integer in [0, budget]")
+    budget = min(budget, cache.k.shape[2])  # a row holds no more
+    recent = min(recent, budget)
     lib = _lib.load()
     size, workspace, pointer = _workspace(cache, budget, lib.fe_evict_workspace_bytes, cache._ref, budget)
     _call(lib.fe_evict_tokens, cache._device_index, cache._ref, out._ref, budget, recent, pointer, size)

@@ -35,3 +35,14 @@ def test_caches_that_take_turns_do_not_keep_each_other():
         assert books[1]() is None
     finally:
         gc.enable()
+
+
+def test_a_budget_past_64_bits_reaches_the_library_as_one_that_holds_everything(monkeypatch):
+    from flash_evict import decode
+    k = torch.zeros(1, 2, 8, 8)
+    cache, sent = host_cache(k, k), []
+    monkeypatch.setattr(decode, "_workspace", lambda cache, key, bytes_of, *args: (0, None, None))
+    monkeypatch.setattr(decode, "_call", lambda fn, device, ref, out, budget, recent, *rest: sent.append((budget, recent)))
+    for budget, recent in ((3, 2), (8, 8), (9, 9), (1 << 40, 7), (2 ** 64 + 1, 0), (2 ** 64 + 2, 2 ** 64 + 1)):
+        assert decode.evict_tokens(cache, budget, recent=recent) is cache
+    assert sent == [(3, 2), (8, 8), (8, 8), (8, 7), (8, 0), (8, 8)]
