@@ -120,11 +120,11 @@ __device__ __forceinline__ int accepted_drafts(const int32_t* accepted, int A, i
   return n;
 }
 
-// Sum over `cols` (a multiple of 16, at most 128) query columns of one key's
+// Sum over `cols` (a multiple of 16, at most 128 / PARTS) query columns of one key's
 // S^T row of exp2(x * sc + bias); `release` is called once the row has been
 // read.  FULL: 128 columns, unrolled.  DRAFT: only columns with bit `bit` of their word in
 // `masks` set.
-template <bool FULL, bool DRAFT, typename Release>
+template <int PARTS, bool FULL, bool DRAFT, typename Release>
 __device__ __forceinline__ float commit_reduce(uint32_t tS, int cols, float sc, const float* bias, const uint32_t* masks,
                                                int bit, Release release) {
   const uint64_t sc2 = f2_pack(sc, sc);
@@ -149,27 +149,47 @@ __device__ __forceinline__ float commit_reduce(uint32_t tS, int cols, float sc, 
       }
     }
   };
-  // The next 16 columns are in flight while these are summed.
-  float xa[16], xb[16];
-  tmem_ld16_nowait(tS, reinterpret_cast<uint32_t*>(xa));
-  tmem_wait_ld16(reinterpret_cast<uint32_t*>(xa));
-  auto pair = [&](int c0, bool more_b, bool more_a) {
-    if (more_b) tmem_ld16_nowait(tS + c0 + 16, reinterpret_cast<uint32_t*>(xb));
-    else release();
-    chunk(c0, xa);
-    if (!more_b) return;
-    tmem_wait_ld16(reinterpret_cast<uint32_t*>(xb));
-    if (more_a) tmem_ld16_nowait(tS + c0 + 32, reinterpret_cast<uint32_t*>(xa));
-    else release();
-    chunk(c0 + 16, xb);
-    if (more_a) tmem_wait_ld16(reinterpret_cast<uint32_t*>(xa));
-  };
-  if (FULL) {
-#pragma unroll
-    for (int c0 = 0; c0 < 128; c0 += 32) pair(c0, true, c0 < 96);
-  } else {
+  if constexpr (PARTS > 1) {
 #pragma unroll 1
-    for (int c0 = 0; c0 < cols; c0 += 32) pair(c0, c0 + 16 < cols, c0 + 32 < cols);
+    for (int c0 = 0; c0 < cols; c0 += 16) {
+      float x[16], y[16];
+      // (Two parts at a time: all four at once would not fit the registers.)
+#pragma unroll
+      for (int i = 0; i < PARTS; i += 2) {
+        float z[16];
+        tmem_ld16_nowait(tS + i * (128 / PARTS) + c0, reinterpret_cast<uint32_t*>(y));
+        tmem_ld16_nowait(tS + (i + 1) * (128 / PARTS) + c0, reinterpret_cast<uint32_t*>(z));
+        tmem_wait_ld16(reinterpret_cast<uint32_t*>(y));
+        tmem_wait_ld16(reinterpret_cast<uint32_t*>(z));
+#pragma unroll
+        for (int c = 0; c < 16; ++c) x[c] = i == 0 ? y[c] + z[c] : x[c] + (y[c] + z[c]);
+      }
+      if (c0 + 16 >= cols) release();
+      chunk(c0, x);
+    }
+  } else {
+    // The next 16 columns are in flight while these are summed.
+    float xa[16], xb[16];
+    tmem_ld16_nowait(tS, reinterpret_cast<uint32_t*>(xa));
+    tmem_wait_ld16(reinterpret_cast<uint32_t*>(xa));
+    auto pair = [&](int c0, bool more_b, bool more_a) {
+      if (more_b) tmem_ld16_nowait(tS + c0 + 16, reinterpret_cast<uint32_t*>(xb));
+      else release();
+      chunk(c0, xa);
+      if (!more_b) return;
+      tmem_wait_ld16(reinterpret_cast<uint32_t*>(xb));
+      if (more_a) tmem_ld16_nowait(tS + c0 + 32, reinterpret_cast<uint32_t*>(xa));
+      else release();
+      chunk(c0 + 16, xb);
+      if (more_a) tmem_wait_ld16(reinterpret_cast<uint32_t*>(xa));
+    };
+    if (FULL) {
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 32) pair(c0, true, c0 < 96);
+    } else {
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols; c0 += 32) pair(c0, c0 + 16 < cols, c0 + 32 < cols);
+    }
   }
   float s[8];
 #pragma unroll
@@ -245,11 +265,17 @@ __device__ __forceinline__ void commit_append_rows(const CommitParams& p, int bh
   }
 }
 
-template <bool BF16, int DP>
+// PARTS: accumulators that a score is summed from, each over a part of the channels
+// and 128 / PARTS columns from the next.  The tensor core cuts its FP32 sums off
+// where an addition would round them, once every 16 channels, so a score leans
+// towards zero, and with it the weights of heavy keys (256 channels in one sum: up to
+// 3.4e-6 off where an FP32 product's are 6e-7); the parts are added in FP32 as usual.
+template <bool BF16, int DP, int PARTS>
 __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
     fe_commit_mass_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tkn,
                           const __grid_constant__ CommitParams p) {
   using C = CommitCfg<DP>;
+  constexpr int CHUNK = 128 / PARTS;  // query columns of a product
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* sbias = reinterpret_cast<float*>(smem + C::OFF_BIAS);
@@ -348,8 +374,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
     const uint32_t dk_lo = static_cast<uint32_t>(dk), dk_hi = static_cast<uint32_t>(dk >> 32);
     const uint32_t dq_lo = static_cast<uint32_t>(dq), dq_hi = static_cast<uint32_t>(dq >> 32);
     uint32_t it0 = 0, nq = 0;
-    uint32_t used[C::WGS];
-    for (int w = 0; w < C::WGS; ++w) used[w] = 0;
+    uint32_t began = 0, parity = 0;  // per warpgroup: has had a product; number of them, mod 2
     bool ok = true;
     while (ok && walk.next(sg)) {
       const int b = sg.bh / p.Hkv;
@@ -359,28 +384,34 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
       if (lane == 0) {
         ok = mbar_wait(q_full, nq & 1, TO, abort_flag);
         tc_fence_after();
-        const int nch = (rows + 127) / 128;
-        // Rounds of one tile per warpgroup; the chunks of 128 queries inside.
-        for (int i0 = 0; i0 < ntile && ok; i0 += C::WGS)
+        constexpr int STEPS = DP / 16 / PARTS;  // of 16 channels a part
+        const int nch = (rows + CHUNK - 1) / CHUNK;
+        // Rounds of a tile per warpgroup, no more than there are stages: they are
+        // kept through the chunks of queries, which are inside.
+        constexpr int ROUND = C::STAGES < C::WGS ? C::STAGES : C::WGS;
+        for (int i0 = 0; i0 < ntile && ok; i0 += ROUND)
           for (int c = 0; c < nch && ok; ++c) {
-            const int cols = (min(rows - c * 128, 128) + 15) & ~15;
+            const int cols = (min(rows - c * CHUNK, CHUNK) + 15) & ~15;
             const uint32_t id = idesc_f16(128, cols, BF16, false);
 #pragma unroll
-            for (int w = 0; w < C::WGS; ++w) {
-              if (i0 + w >= ntile || !ok) continue;
-              const uint32_t tile = it0 + i0 + w;
+            for (int u = 0; u < ROUND; ++u) {
+              if (i0 + u >= ntile || !ok) continue;
+              const int w = (i0 + u) % C::WGS;
+              const uint32_t tile = it0 + i0 + u;
               const int s = tile % C::STAGES;
               if (c == 0) ok = mbar_wait(&k_full[s], (tile / C::STAGES) & 1, TO, abort_flag);
-              if (ok && used[w] > 0) ok = mbar_wait(&s_free[w], (used[w] - 1) & 1, TO, abort_flag);
+              if (ok && ((began >> w) & 1u)) ok = mbar_wait(&s_free[w], ((parity >> w) & 1u) ^ 1u, TO, abort_flag);
               if (!ok) continue;
-              ++used[w];
+              began |= 1u << w;
+              parity ^= 1u << w;
               tc_fence_after();
               const uint32_t ka = dk_lo + static_cast<uint32_t>(s * (C::TILE >> 4));
-              const uint32_t qa = dq_lo + static_cast<uint32_t>(c * (C::TILE >> 4));
+              const int row = c * CHUNK;
+              const uint32_t qa = dq_lo + static_cast<uint32_t>((row >> 7) * (C::TILE >> 4) + (row & 127) * (128 >> 4));
 #pragma unroll
               for (int kk = 0; kk < DP / 16; ++kk) {
                 const uint32_t off = static_cast<uint32_t>(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
-                umma_ss_lohi(tmem + w * 128, ka + off, dk_hi, qa + off, dq_hi, id, kk > 0);
+                umma_ss_lohi(tmem + w * 128 + kk / STEPS * CHUNK, ka + off, dk_hi, qa + off, dq_hi, id, kk % STEPS != 0);
               }
               umma_commit(&s_full[w]);
               if (c == nch - 1) umma_commit(&k_empty[s]);
@@ -511,7 +542,7 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
         if (lane == 0) mbar_arrive(q_full);
         named_bar_sync(1, RT);
       }
-      const int nch = (rows + 127) / 128;
+      const int nch = (rows + CHUNK - 1) / CHUNK;
       for (int i = wg; i < ntile; i += C::WGS) {
         const int j = sg.j0 + i;
         const bool drafts = j == sg.tiles - 1;
@@ -536,19 +567,19 @@ __global__ void __launch_bounds__(CommitCfg<DP>::THREADS, 1)
           if (!ok) break;
           ++li;
           tc_fence_after();
-          const int cols = (min(rows - c * 128, 128) + 15) & ~15;
+          const int cols = (min(rows - c * CHUNK, CHUNK) + 15) & ~15;
           auto release = [&] {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[wg]);
           };
-          const float* bias = sbias + c * 128;
+          const float* bias = sbias + c * CHUNK;
           if (drafts)
-            total += commit_reduce<false, true>(tS, cols, p.sc, bias, scol + (kr >> 5) * C::ROWS + c * 128, kr & 31, release);
-          else if (cols == 128)
-            total += commit_reduce<true, false>(tS, cols, p.sc, bias, nullptr, 0, release);
+            total += commit_reduce<PARTS, false, true>(tS, cols, p.sc, bias, scol + (kr >> 5) * C::ROWS + c * CHUNK, kr & 31, release);
+          else if (PARTS == 1 && cols == 128)
+            total += commit_reduce<PARTS, true, false>(tS, cols, p.sc, bias, nullptr, 0, release);
           else
-            total += commit_reduce<false, false>(tS, cols, p.sc, bias, nullptr, 0, release);
+            total += commit_reduce<PARTS, false, false>(tS, cols, p.sc, bias, nullptr, 0, release);
         }
         // Aborted (watchdog): the sum is incomplete; store NaN.
         if (!ok) total = __int_as_float(0x7fffffff);

@@ -352,10 +352,10 @@ int64_t commit_workspace(const fe_cache* c, bool in_place, int64_t q_heads, int6
   return *off_lengths + (in_place ? nbh * 4 : 0);
 }
 
-template <bool BF16, int DP>
-int launch_commit(const CUtensorMap& tk, const CUtensorMap& tkn, fe::CommitParams p, cudaStream_t stream) {
+template <bool BF16, int DP, int PARTS>
+int launch_commit_parts(const CUtensorMap& tk, const CUtensorMap& tkn, fe::CommitParams p, cudaStream_t stream) {
   using C = fe::CommitCfg<DP>;
-  auto kern = fe::fe_commit_mass_kernel<BF16, DP>;
+  auto kern = fe::fe_commit_mass_kernel<BF16, DP, PARTS>;
   int rc = set_smem(kern, C::SMEM);
   if (rc) return rc;
   static std::atomic<int> checked_regs{0};
@@ -372,6 +372,22 @@ int launch_commit(const CUtensorMap& tk, const CUtensorMap& tkn, fe::CommitParam
     if (rc) return rc;
   }
   return FE_STATUS_OK;
+}
+
+// As many parts to a score (see the kernel) as leave 128 columns for the queries;
+// 256 channels always four.  Equally heavy fp16 keys of score 40 lean by 5.0e-5 with
+// 256 channels in one sum, 1.8e-5 in two, under 7.2e-6 in four.  That costs their runs
+// of more than 32 queries time (256 over 65536 tokens: one sum 115 us, two 137, four
+// 227); up to 128 channels (1.8e-5 in one sum) longer runs keep one (256 queries over
+// 131072 tokens: 92 us, two sums 138).
+template <bool BF16, int DP>
+int launch_commit(const CUtensorMap& tk, const CUtensorMap& tkn, const fe::CommitParams& p, cudaStream_t stream) {
+  const int64_t rows = (int64_t)p.A * p.G;
+  if constexpr (DP <= 128) {
+    if (rows > 64) return launch_commit_parts<BF16, DP, 1>(tk, tkn, p, stream);
+    if (rows > 32) return launch_commit_parts<BF16, DP, 2>(tk, tkn, p, stream);
+  }
+  return launch_commit_parts<BF16, DP, 4>(tk, tkn, p, stream);
 }
 
 }  // namespace

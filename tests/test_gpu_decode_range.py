@@ -57,3 +57,35 @@ def test_keys_of_minus_infinite_score_add_nothing(dtype, hq, hk, d, t, took):
     # the accepted queries' weights add up to one each (2^-18: as for the mass in test_gpu_decode_cache)
     # but for what goes to drafts that were not accepted, which none of these sees
     assert ((live.sum(-1) - mass[:, :, :n].sum(-1) - took * (hq // hk)).abs() <= 2.0 ** -18 * live.sum(-1)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,hq,t,parts", [(256, 1, 1, 4), (256, 40, 2, 2), (128, 4, 1, 4)])
+def test_committed_weights_do_not_lean(dtype, d, hq, t, parts):
+    """The mean error of equally heavy keys' weights, whose random part averages out.
+
+    A sum of 16 channels cut off to FP32 loses half a last place on average, at most
+    2^-24 of the sum so far; over a part's d / 16 / parts steps, with terms of one sign
+    and size, that is (steps + 1) / 2 * 2^-24 of the score.  Half a unit more covers
+    the rounding of scale * log2(e) and ex2.  (parts: the fewest that a score may be
+    summed in.)
+    """
+    n, scale = 4096, 1 / 16
+    gen = torch.Generator().manual_seed(63)
+    spread = lambda *shape: (1 + 0.3 * (2 * torch.rand(*shape, generator=gen) - 1)) * (40 / (scale * d)) ** 0.5  # noqa: E731
+    q, k, kn = (spread(1, h, m, d).to(dtype).cuda() for h, m in ((hq, t), (1, n + 2), (1, t)))
+    vn = torch.zeros_like(kn)
+    s = scale * (q[0].double() @ k[0, 0, :n].double().T)  # [hq, t, n]
+    # row sums whose product with log2(e) FP32 holds exactly, or nearly
+    near = (s.mean() + math.log(n)).float() * (1 + torch.arange(4096, device="cuda") * 2.0 ** -23).float()
+    bias = near.double() * math.log2(math.e)
+    lse = near[(bias - bias.float().double()).abs().argmin()].expand(1, hq, t).contiguous()
+    book = (torch.full((1, 1), n, dtype=torch.int32, device="cuda"), torch.zeros(1, 1, n + 2, device="cuda"),
+            torch.zeros(1, 1, n + 2, dtype=torch.int32, device="cuda"))
+    cache = KVCache(k, torch.zeros_like(k), *book)
+    accepted = torch.arange(t, dtype=torch.int32, device="cuda")[None]
+    commit_tokens(cache, q, kn, vn, lse, accepted, torch.full((1, t), n, dtype=torch.int32, device="cuda"), scale=scale)
+    want = torch.exp(s - lse[0, 0, 0].double()).sum((0, 1))
+    lean = (cache.mass[0, 0, :n].double() / want - 1).mean().item()
+    steps = d // 16 // parts
+    assert abs(lean) <= ((steps + 1) / 2 + 0.5) * 2.0 ** -24 * s.mean().item(), lean / (2.0 ** -24 * s.mean().item())
