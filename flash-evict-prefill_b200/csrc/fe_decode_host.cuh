@@ -107,7 +107,8 @@ int tree_geometry(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t draf
   g->ctas = std::min<int64_t>(sms, nbh * g->MT * tiles);
   // A cluster of eight per item instead of all SMs and a second launch: about
   // 4 us less, for (tiles/8 - items*tiles/SMs) more tiles of 1.2 us in a row.
-  // (8 rows, one token: 4000 keys 13.2 us against 16, 6000 keys 16.1 for both.)
+  // (8 rows, one token: 4000 keys 12.1 us against 16.6, 6000 keys 13.9 and 15.2,
+  // 8000 keys 16.5 and 17.1.)
   const int64_t items = nbh * g->MT;
   g->cluster = !g->dual && items * (fe::TREE_CLUSTER + 1) <= sms &&
                2 * tiles * (sms - items * fe::TREE_CLUSTER) <= 7 * fe::TREE_CLUSTER * sms;
@@ -365,8 +366,8 @@ int launch_commit_parts(const CUtensorMap& tk, const CUtensorMap& tkn, fe::Commi
     p.row0 = (int)row0;
     p.last = row0 + C::ROWS >= (int64_t)p.A * p.G;
     // A row begins with the gather of its queries: two key tiles' time, and one
-    // more for every 64 of them (batch of 16, 4 rows: 35.5 us with none, 33.0 with
-    // 2; 256 rows over 131k 108, 104, and 99 with 5).
+    // more for every 64 of them (batch of 16, 4 rows: 31.5 us with none, 29.6 with
+    // 2; 256 rows over 131k 100, 97, and 92 with 6).
     p.extra = 2 + (int)(std::min<int64_t>((int64_t)p.A * p.G - row0, C::ROWS) / 64);
     rc = launch_dependent(kern, dim3((unsigned)p.nctas), dim3(C::THREADS), C::SMEM, 1, stream, "commit launch", tk, tkn, p);
     if (rc) return rc;

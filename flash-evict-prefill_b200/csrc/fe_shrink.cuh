@@ -15,7 +15,8 @@
 // One cluster of CTAs per row, every warp a contiguous stretch of slots whose
 // order-preserving integer keys stay in shared memory (in registers the walks
 // over them have to be unrolled, and fetching that code once took longer than
-// running it: 46 us instead of 40 for eight rows of 128K, all else alike).  The budget-th largest key is
+// running it: 46 us instead of 40 for eight rows of 128K when that was all that
+// differed; the whole takes 28 now).  The budget-th largest key is
 // found by narrowing the range of the keys 1024-fold a pass (bins of a power of
 // two from the row's smallest key, so keys that share their top bits spread over
 // the bins all the same), histograms summed over distributed shared memory,

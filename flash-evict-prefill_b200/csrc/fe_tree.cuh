@@ -18,7 +18,7 @@
 // joins them in a fixed order (no atomics, bitwise reproducible).  Few short
 // rows (a decode step over compacted caches) are latency instead: there a
 // cluster of eight CTAs has a row and joins through distributed shared memory,
-// in one launch (CLUSTER; 12.4 -> 10.7 us for 4 rows of 2048).
+// in one launch (CLUSTER; 9.9 us for 4 rows of 2048, 11.3 the other way).
 //
 // Roles (384 threads): warps 0-3 and 4-7 are two softmax warpgroups, warp 8
 // issues TMA, warp 9 tcgen05.mma.  Up to 128 rows (SPLIT) both warpgroups
@@ -91,8 +91,8 @@ constexpr float TREE_HEADROOM = BF16 ? 0.0f : 7.0f;
 // Lowest running max: finite, so that a row which has seen no key yet rescales
 // by 2^-huge = 0 and never forms inf - inf.
 constexpr float TREE_M0 = -3.0e38f;
-// Key tiles that beginning and ending a row cost (batch of 16: 61.6 us with none,
-// 58.2, 54.9, 53.8 and 53.3 with 1 to 4; 64 drafts over 32k 53.7, 51.2, 49.6, 50.4, 50.2).
+// Key tiles that beginning and ending a row cost (batch of 16: 58.8 us with none,
+// 56.1, 53.7, 53.1 and 53.7 with 1 to 4; 64 drafts over 32k 57.0, 54.9, 52.4, 52.4, 52.3).
 constexpr int TREE_EXTRA = 3;
 constexpr uint32_t TREE_QBUF = 8192;  // bytes between the halves of a query tile's 64-column group
 
@@ -763,7 +763,7 @@ __global__ void __launch_bounds__(TREE_JOIN_THREADS)
   const int quad0 = live ? pair / rows * Q : 0, r = live ? pair % rows : 0;
   // Which runs had the row.  (The kernel before the attention may have written
   // the lengths and still be running until here: the attention lets this one
-  // start ahead of its own wait.)
+  // start ahead of its own wait.  Of 64 drafts over 32k, 52.4 us, it costs about 1.)
   pdl_wait();
   int first, last, start;
   const DecLayout d = dec_layout<TREE_JOIN_THREADS>(p.lengths, p.B * p.Hkv, p.capacity, p.MT, TREE_EXTRA, p.nctas, scratch,
